@@ -267,6 +267,122 @@ knng_gpu_status knng_gpu_brute_force_multi(const float* data, uint64_t n, uint64
                                            knng_gpu_stats* stats);
 void knng_gpu_release_multi(void);
 
+/* ---- projection and softmax loss on device rows ---------------------------
+ * The step before a search: a linear layer that makes the rows, and the
+ * softmax over inner products with a large set of rows that trains it. No
+ * counterpart in the reference.
+ *
+ * All pointers are device pointers, matrices are row-major with a row stride
+ * `ld*` in elements (>= the row's width), calls are asynchronous on `stream`
+ * and allocate no device memory: the caller passes a workspace of
+ * knng_gpu_*_workspace_bytes (same arguments) bytes, 256-byte aligned, that
+ * it may reuse once the stream has passed the call. Outputs must not overlap
+ * inputs. Sums, softmax statistics and accumulators are fp32. fp32 operands
+ * are multiplied as three bf16 parts each (products down to 2^-18 of the
+ * leading one, fp32 sums); an infinity there gives NaN. A bounded
+ * device-side wait that gives up is reported as KNNG_GPU_TIMEOUT by the next
+ * of these calls. */
+typedef enum { KNNG_DTYPE_F32 = 0, KNNG_DTYPE_BF16 = 1, KNNG_DTYPE_F16 = 2 } knng_dtype;
+typedef enum {
+    KNNG_ACT_NONE = 0,
+    KNNG_ACT_RELU = 1,
+    KNNG_ACT_GELU = 2,      /* z Phi(z) */
+    KNNG_ACT_GELU_TANH = 3, /* its tanh form */
+    KNNG_ACT_SILU = 4
+} knng_activation;
+
+/* out = act(x w^T + bias) + residual: x (m, k), w (n, k), bias (n),
+ * residual and out (m, n). bias, residual and pre may be NULL; pre receives
+ * x w^T + bias. Everything has type dtype, out dtype or fp32. */
+typedef struct {
+    uint64_t m, k, n;
+    const void* x;
+    uint64_t ldx;
+    const void* w;
+    uint64_t ldw;
+    const void* bias;
+    const void* residual;
+    uint64_t ldr;
+    void* out;
+    uint64_t ldo;
+    void* pre;
+    uint64_t ldp;
+    int dtype;
+    int out_dtype;
+    int activation;
+} knng_gpu_linear_args;
+uint64_t knng_gpu_linear_workspace_bytes(const knng_gpu_linear_args* a);
+knng_gpu_status knng_gpu_linear(const knng_gpu_linear_args* a, void* d_workspace, uint64_t workspace_bytes,
+                                void* stream);
+
+/* Gradients of the linear layer: dz = dy act'(pre) (pre may be NULL without
+ * activation), dx = dz w, dw = dz^T x, db = column sums of dz. dx (m, k),
+ * dw (n, k) and db (n), each dense and each possibly NULL (not wanted). */
+typedef struct {
+    uint64_t m, k, n;
+    const void* dy;
+    uint64_t lddy;
+    const void* x;
+    uint64_t ldx;
+    const void* w;
+    uint64_t ldw;
+    const void* pre;
+    uint64_t ldp;
+    void* dx;
+    void* dw;
+    void* db;
+    int dtype;
+    int activation;
+} knng_gpu_linear_backward_args;
+uint64_t knng_gpu_linear_backward_workspace_bytes(const knng_gpu_linear_backward_args* a);
+knng_gpu_status knng_gpu_linear_backward(const knng_gpu_linear_backward_args* a, void* d_workspace,
+                                         uint64_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy over inner products, without the (m, n) scores:
+ * z_ij = scale x_i . w_j, lse_i = log sum_j exp z_ij, loss_i = lse_i - z_i,y_i.
+ * x (m, k) and w (n, k) of type dtype, labels int64 or int32, loss and lse
+ * fp32 (m). A label outside [0, n) leaves its row out: loss 0. scale > 0. */
+typedef struct {
+    uint64_t m, k, n;
+    const void* x;
+    uint64_t ldx;
+    const void* w;
+    uint64_t ldw;
+    const void* labels;
+    float* loss;
+    float* lse;
+    float scale;
+    int dtype;
+    int labels_i64;
+} knng_gpu_softmax_xent_args;
+uint64_t knng_gpu_softmax_xent_workspace_bytes(const knng_gpu_softmax_xent_args* a);
+knng_gpu_status knng_gpu_softmax_xent(const knng_gpu_softmax_xent_args* a, void* d_workspace,
+                                      uint64_t workspace_bytes, void* stream);
+
+/* Its gradients from lse: g_ij = dloss_i scale (exp(z_ij - lse_i) - [j = y_i]),
+ * dx = g w, dw = g^T x (dense, of type dtype). A row without a label adds
+ * nothing to dw, whatever it holds, and its dx is 0. g is recomputed for a
+ * piece of w at a time and kept in bf16/fp16 relative to the largest |dloss|
+ * (three bf16 parts for fp32). */
+typedef struct {
+    uint64_t m, k, n;
+    const float* dloss;
+    const void* x;
+    uint64_t ldx;
+    const void* w;
+    uint64_t ldw;
+    const void* labels;
+    const float* lse;
+    void* dx;
+    void* dw;
+    float scale;
+    int dtype;
+    int labels_i64;
+} knng_gpu_softmax_xent_backward_args;
+uint64_t knng_gpu_softmax_xent_backward_workspace_bytes(const knng_gpu_softmax_xent_backward_args* a);
+knng_gpu_status knng_gpu_softmax_xent_backward(const knng_gpu_softmax_xent_backward_args* a, void* d_workspace,
+                                               uint64_t workspace_bytes, void* stream);
+
 /* ---- test hook -----------------------------------------------------------
  * Runs one small build whose device-side waits give up after
  * `wait_limit_cycles` clock cycles while the kernel's producer withholds one

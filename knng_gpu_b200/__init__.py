@@ -30,3 +30,9 @@ from .api import (  # noqa: F401
     recall_at_k,
     workspace_bytes,
 )
+from .learn import (  # noqa: F401
+    linear,
+    linear_backward,
+    softmax_xent,
+    softmax_xent_backward,
+)

@@ -48,6 +48,14 @@ GPU_SYMBOLS = (
     "knng_gpu_knn_f32_sets_scratch_bytes",
     "knng_gpu_knn_f32_sets",
     "knng_gpu_recall_at_k",
+    "knng_gpu_linear_workspace_bytes",
+    "knng_gpu_linear",
+    "knng_gpu_linear_backward_workspace_bytes",
+    "knng_gpu_linear_backward",
+    "knng_gpu_softmax_xent_workspace_bytes",
+    "knng_gpu_softmax_xent",
+    "knng_gpu_softmax_xent_backward_workspace_bytes",
+    "knng_gpu_softmax_xent_backward",
 )
 
 
@@ -68,6 +76,52 @@ class KnngGpuStats(ctypes.Structure):
 
     def as_dict(self) -> dict:
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+class LinearArgs(ctypes.Structure):
+    """Mirror of ``knng_gpu_linear_args``."""
+
+    _fields_ = [
+        ("m", c_uint64), ("k", c_uint64), ("n", c_uint64),
+        ("x", c_void_p), ("ldx", c_uint64), ("w", c_void_p), ("ldw", c_uint64),
+        ("bias", c_void_p), ("residual", c_void_p), ("ldr", c_uint64),
+        ("out", c_void_p), ("ldo", c_uint64), ("pre", c_void_p), ("ldp", c_uint64),
+        ("dtype", c_int), ("out_dtype", c_int), ("activation", c_int),
+    ]
+
+
+class LinearBackwardArgs(ctypes.Structure):
+    """Mirror of ``knng_gpu_linear_backward_args``."""
+
+    _fields_ = [
+        ("m", c_uint64), ("k", c_uint64), ("n", c_uint64),
+        ("dy", c_void_p), ("lddy", c_uint64), ("x", c_void_p), ("ldx", c_uint64),
+        ("w", c_void_p), ("ldw", c_uint64), ("pre", c_void_p), ("ldp", c_uint64),
+        ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p),
+        ("dtype", c_int), ("activation", c_int),
+    ]
+
+
+class SoftmaxXentArgs(ctypes.Structure):
+    """Mirror of ``knng_gpu_softmax_xent_args``."""
+
+    _fields_ = [
+        ("m", c_uint64), ("k", c_uint64), ("n", c_uint64),
+        ("x", c_void_p), ("ldx", c_uint64), ("w", c_void_p), ("ldw", c_uint64),
+        ("labels", c_void_p), ("loss", c_void_p), ("lse", c_void_p),
+        ("scale", c_float), ("dtype", c_int), ("labels_i64", c_int),
+    ]
+
+
+class SoftmaxXentBackwardArgs(ctypes.Structure):
+    """Mirror of ``knng_gpu_softmax_xent_backward_args``."""
+
+    _fields_ = [
+        ("m", c_uint64), ("k", c_uint64), ("n", c_uint64),
+        ("dloss", c_void_p), ("x", c_void_p), ("ldx", c_uint64), ("w", c_void_p), ("ldw", c_uint64),
+        ("labels", c_void_p), ("lse", c_void_p), ("dx", c_void_p), ("dw", c_void_p),
+        ("scale", c_float), ("dtype", c_int), ("labels_i64", c_int),
+    ]
 
 
 _gpu = None
@@ -147,6 +201,10 @@ def gpu_lib() -> ctypes.CDLL:
                  c_uint64, c_void_p, st],
             ),
         }
+        for name, args in (("linear", LinearArgs), ("linear_backward", LinearBackwardArgs),
+                           ("softmax_xent", SoftmaxXentArgs), ("softmax_xent_backward", SoftmaxXentBackwardArgs)):
+            sig[f"knng_gpu_{name}_workspace_bytes"] = (c_uint64, [POINTER(args)])
+            sig[f"knng_gpu_{name}"] = (c_int, [POINTER(args), c_void_p, c_uint64, c_void_p])
         del f32p, u32p, i32p
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)

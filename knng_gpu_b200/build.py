@@ -35,11 +35,31 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 def build_gpu(verbose: bool = False, force: bool = False) -> Path:
     out = PKG / "libknng_gpu.so"
-    srcs = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "knng_gpu.h"]
-    if force or _stale(out, srcs):
+    units = {
+        "knng_gpu.cu": ["internal.hpp", "knn_exact.cuh", "knn_pair.cuh", "knn_rerank.cuh", "knn_tc.cuh", "ptx.cuh",
+                        "schedule.cuh", "sharded.cuh", "topk.cuh"],
+        "learn.cu": ["internal.hpp", "learn.cuh", "product.cuh", "ptx.cuh"],
+    }
+    sources = {name: [CSRC / name, *(CSRC / p for p in parts), ROOT / "include" / "knng_gpu.h"]
+               for name, parts in units.items()}
+    if force or any(_stale(out, srcs) for srcs in sources.values()):
+        obj_dir = CSRC / "_build"
+        obj_dir.mkdir(exist_ok=True)
+        objs, jobs = [], []
+        for name, srcs in sources.items():
+            obj = obj_dir / (Path(name).stem + ".o")
+            objs.append(str(obj))
+            if force or _stale(obj, srcs):
+                cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-c",
+                       f"-I{ROOT / 'include'}", "-o", str(obj), str(CSRC / name)]
+                if verbose:
+                    print(" ".join(cmd), flush=True)
+                jobs.append((cmd, subprocess.Popen(cmd)))
+        failed = [cmd for cmd, job in jobs if job.wait() != 0]
+        if failed:
+            raise subprocess.CalledProcessError(1, failed[0])
         tmp = out.with_suffix(".so.tmp")
-        _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-shared",
-              f"-I{ROOT / 'include'}", "-o", str(tmp), str(CSRC / "knng_gpu.cu"), "-lnccl"], verbose)
+        _run([NVCC, *ARCH, "-shared", "-o", str(tmp), *objs, "-lnccl"], verbose)
         tmp.replace(out)
     return out
 

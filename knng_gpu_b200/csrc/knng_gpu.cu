@@ -17,6 +17,7 @@
 #include <thread>
 #include <vector>
 
+#include "internal.hpp"
 #include "knn_exact.cuh"
 #include "knn_pair.cuh"
 #include "knn_rerank.cuh"
@@ -1593,6 +1594,9 @@ knng_gpu_status grow(void** ptr, uint64_t* cap, uint64_t need)
     return KNNG_GPU_OK;
 }
 }  // namespace
+
+knng_gpu_status knng_b200::set_last_error(knng_gpu_status s, const std::string& msg) { return fail(s, msg); }
+void knng_b200::clear_last_error() { g_last_error.clear(); }
 
 extern "C" {
 

@@ -1,0 +1,860 @@
+// learn.cu -- C-ABI entry points of the projection and the softmax loss over
+// inner products (include/knng_gpu.h) and their host-side orchestration.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <mutex>
+#include <string>
+
+#include "internal.hpp"
+#include "knng_gpu.h"
+#include "learn.cuh"
+
+using namespace knng_b200;
+
+namespace {
+
+knng_gpu_status fail(knng_gpu_status s, const std::string& msg) { return set_last_error(s, msg); }
+
+#define KNNG_CUDA(call)                                                                          \
+    do {                                                                                         \
+        cudaError_t e_ = (call);                                                                 \
+        if (e_ != cudaSuccess)                                                                   \
+            return fail(e_ == cudaErrorMemoryAllocation ? KNNG_GPU_OUT_OF_MEMORY : KNNG_GPU_CUDA_ERROR, \
+                        std::string("knng::gpu: ") + #call + ": " + cudaGetErrorString(e_));     \
+    } while (0)
+
+#define KNNG_TRY(expr)                        \
+    do {                                      \
+        knng_gpu_status s_ = (expr);          \
+        if (s_ != KNNG_GPU_OK) return s_;     \
+    } while (0)
+
+constexpr uint64_t up(uint64_t x, uint64_t a) { return (x + a - 1) / a * a; }
+constexpr uint64_t ceil_div(uint64_t x, uint64_t a) { return (x + a - 1) / a; }
+
+uint32_t elem_bytes(int dtype) { return dtype == KNNG_DTYPE_F32 ? 4 : 2; }
+
+// Number of bytes a call would need (base NULL), or the pieces of a workspace.
+struct Carver {
+    uint8_t* base;
+    uint64_t at = 0;
+    explicit Carver(void* b) : base(static_cast<uint8_t*>(b)) {}
+    template <class T>
+    T* take(uint64_t count)
+    {
+        T* p = base ? reinterpret_cast<T*>(base + at) : nullptr;
+        at = up(at + count * sizeof(T), 256);
+        return p;
+    }
+};
+
+// ------------------------------------------------------------------ device facts
+// Error word of the product kernel: host memory that kernels can write, so an
+// asynchronous call needs no synchronisation to report a wait that gave up.
+knng_gpu_status error_word(int** out)
+{
+    static std::mutex mu;
+    static int* word = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!word) {
+        void* p = nullptr;
+        KNNG_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+        word = static_cast<int*>(p);
+        *word = 0;
+    }
+    *out = word;
+    return KNNG_GPU_OK;
+}
+
+knng_gpu_status take_error(int** word)
+{
+    KNNG_TRY(error_word(word));
+    if (reinterpret_cast<std::atomic<int>*>(*word)->exchange(0) != 0)
+        return fail(KNNG_GPU_TIMEOUT, "knng::gpu: a bounded device wait gave up in an earlier call on device rows");
+    return KNNG_GPU_OK;
+}
+
+uint32_t sm_count()
+{
+    static std::atomic<uint32_t> cached{0};
+    uint32_t n = cached.load(std::memory_order_relaxed);
+    if (n == 0) {
+        int dev = 0, sms = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        n = sms > 0 ? static_cast<uint32_t>(sms) : 148u;
+        if (sms > 0) cached.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// ------------------------------------------------------------------ maps
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+knng_gpu_status encode_fn(EncodeTiledFn* out)
+{
+    static std::atomic<void*> cached{nullptr};
+    void* p = cached.load(std::memory_order_acquire);
+    if (!p) {
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !p)
+            return fail(KNNG_GPU_CUDA_ERROR, "knng::gpu: cuTensorMapEncodeTiled entry point not available");
+        cached.store(p, std::memory_order_release);
+    }
+    *out = reinterpret_cast<EncodeTiledFn>(p);
+    return KNNG_GPU_OK;
+}
+
+// rows x width elements at stride `ld`; boxes of box_w x box_h elements,
+// swizzled over their width of 64 or 128 bytes; zeros past the ends.
+knng_gpu_status make_map(CUtensorMap* map, int type, const void* base, uint64_t width, uint64_t rows, uint64_t ld,
+                         uint32_t box_w, uint32_t box_h)
+{
+    EncodeTiledFn enc;
+    KNNG_TRY(encode_fn(&enc));
+    const uint32_t e = elem_bytes(type);
+    const CUtensorMapDataType dt = type == KNNG_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : type == KNNG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t dims[2] = {width, rows};
+    const cuuint64_t strides[1] = {ld * e};
+    const cuuint32_t box[2] = {box_w, box_h};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapSwizzle sw = box_w * e == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    const CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(KNNG_GPU_CUDA_ERROR, "knng::gpu: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return KNNG_GPU_OK;
+}
+
+// TMA reads and writes rows that start on 16-byte boundaries.
+bool tma_rows(const void* p, uint64_t ld, uint32_t e)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * e) % 16 == 0;
+}
+
+// ------------------------------------------------------------------ operands
+// A matrix that the product reads: `rows` stored rows of `width` 16-bit
+// elements (all planes), `ld` apart.
+struct Operand {
+    const void* ptr;
+    uint64_t rows, width, ld;
+    uint32_t plane;  // columns from one plane to the next
+};
+
+struct Source {  // a caller's matrix
+    const void* ptr;
+    uint64_t rows, k, ld;
+};
+
+bool needs_stage(const Source& s, int dtype) { return dtype == KNNG_DTYPE_F32 || !tma_rows(s.ptr, s.ld, 2); }
+uint32_t planes_of(int dtype) { return dtype == KNNG_DTYPE_F32 ? 3u : 1u; }
+// Columns of a staged plane: 16-byte rows; whole K blocks where planes lie side by side.
+uint64_t stage_pitch(uint64_t k, int dtype) { return dtype == KNNG_DTYPE_F32 ? up(k, 64) : up(k, 8); }
+
+uint64_t stage_elems(const Source& s, int dtype) { return s.rows * stage_pitch(s.k, dtype) * planes_of(dtype); }
+
+struct RowLabels {
+    const void* ptr = nullptr;
+    int i64 = 0;
+    uint32_t classes = 0;
+};
+
+knng_gpu_status stage(const Source& s, int dtype, uint16_t* dst, Operand* out, cudaStream_t st,
+                      const RowLabels& labels = RowLabels())
+{
+    const uint64_t pitch = stage_pitch(s.k, dtype);
+    const uint64_t blocks = std::min<uint64_t>(ceil_div(s.rows * (pitch / 8), 256), 148ull * 16);
+    if (dtype == KNNG_DTYPE_F32)
+        stage_rows_kernel<3><<<static_cast<uint32_t>(blocks), 256, 0, st>>>(
+            s.ptr, s.rows, static_cast<uint32_t>(s.k), s.ld, dst, static_cast<uint32_t>(pitch), labels.ptr, labels.i64,
+            labels.classes);
+    else
+        stage_rows_kernel<1><<<static_cast<uint32_t>(blocks), 256, 0, st>>>(
+            s.ptr, s.rows, static_cast<uint32_t>(s.k), s.ld, dst, static_cast<uint32_t>(pitch), labels.ptr, labels.i64,
+            labels.classes);
+    KNNG_CUDA(cudaGetLastError());
+    const uint32_t planes = planes_of(dtype);
+    *out = Operand{dst, s.rows, pitch * planes, pitch * planes, static_cast<uint32_t>(pitch)};
+    return KNNG_GPU_OK;
+}
+
+Operand direct(const Source& s) { return Operand{s.ptr, s.rows, s.k, s.ld, 0}; }
+
+// The operand as the product reads it: staged through `dst` where needed.
+knng_gpu_status operand(const Source& s, int dtype, uint16_t* dst, Operand* out, cudaStream_t st)
+{
+    if (needs_stage(s, dtype)) return stage(s, dtype, dst, out, st);
+    *out = direct(s);
+    return KNNG_GPU_OK;
+}
+
+// ------------------------------------------------------------------ product launches
+struct Shape {
+    uint64_t m, n, k;
+    uint32_t combos;
+    bool precise;  // the result is kept in fp32
+};
+
+// Longest K summed by the tensor cores alone (their additions truncate): 128
+// where fp32 comes of it, 1024 where 16 bits do. Against 64 bits, lse of fp16
+// rows of width 785 is off by 1.9e-6 of its size when K is summed in one
+// piece and by 1.9e-7 in pieces of 128 (plain fp32: 0.8e-7); a 16-bit result
+// has 2e-4 or more of its own.
+constexpr uint32_t kPreciseBlocks = 2, kShortBlocks = 16;
+
+struct Plan {
+    int cg;
+    uint32_t tiles_m, tiles_n, kblocks, splits, piece;
+    uint32_t pieces() const { return (kblocks + piece - 1) / piece; }
+    uint64_t split_rows, part_pitch;  // of the fp32 pieces of a split product
+    uint64_t part_elems() const { return splits > 1 ? splits * split_rows * part_pitch : 0; }
+};
+
+Plan tiles_of(const Shape& s, int cg)
+{
+    Plan q;
+    q.cg = cg;
+    q.tiles_m = static_cast<uint32_t>(ceil_div(s.m, 128 * cg));
+    q.tiles_n = static_cast<uint32_t>(ceil_div(s.n, 128 * cg));
+    q.kblocks = static_cast<uint32_t>(ceil_div(s.k, 64));
+    q.splits = 1;
+    q.piece = std::min(q.kblocks, s.precise ? kPreciseBlocks : kShortBlocks);
+    q.split_rows = uint64_t(q.tiles_m) * 128 * cg;
+    q.part_pitch = uint64_t(q.tiles_n) * 128 * cg;
+    return q;
+}
+
+// Pairs (256 x 256 tiles) once they occupy most of the GPU, otherwise 128 x 128
+// tiles; with fewer tiles than SMs the K loop is cut so that the pieces fill
+// the SMs, down to four K blocks a piece.
+Plan plan_product(const Shape& s)
+{
+    const Plan pair = tiles_of(s, 2);
+    if (uint64_t(pair.tiles_m) * pair.tiles_n * 2 >= sm_count() * 3ull / 4) return pair;
+    Plan q = tiles_of(s, 1);
+    const uint64_t tiles = uint64_t(q.tiles_m) * q.tiles_n;
+    if (tiles < sm_count()) {
+        const uint64_t least = ceil_div(4, s.combos);  // K blocks
+        const uint64_t want = std::max<uint64_t>(1, std::min<uint64_t>(sm_count() / tiles, q.kblocks / least));
+        q.piece = static_cast<uint32_t>(std::min<uint64_t>(q.piece, ceil_div(q.kblocks, want)));
+        q.splits = static_cast<uint32_t>(std::min<uint64_t>(want, q.pieces()));
+    }
+    return q;
+}
+
+template <int CG, bool AMN, bool BMN, int EPI, bool LONG>
+knng_gpu_status launch_product_t(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const CUtensorMap& pre,
+                               const ProductParams& p, cudaStream_t st)
+{
+    auto* kern = product_kernel<CG, AMN, BMN, EPI, LONG>;
+    // Units that fit the device at once (the same on every GPU this library is built for).
+    static std::atomic<uint32_t> fit{0};
+    uint32_t units = fit.load(std::memory_order_acquire);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kPkThreads);
+    cfg.dynamicSmemBytes = kPkSmem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    KNNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPkSmem));
+    if (units == 0) {
+        units = sm_count() / CG;
+        if (CG == 2) {
+            int clusters = 0;
+            cfg.gridDim = dim3(sm_count() / 2 * 2);
+            KNNG_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
+            units = static_cast<uint32_t>(std::max(1, std::min<int>(clusters, static_cast<int>(units))));
+        }
+        fit.store(units, std::memory_order_release);
+    }
+    cfg.gridDim = dim3(std::min(units, p.items) * CG);
+    KNNG_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b, o, pre, p));
+    return KNNG_GPU_OK;
+}
+
+template <int CG, bool AMN, bool BMN, int EPI>
+knng_gpu_status launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const CUtensorMap& pre,
+                               const ProductParams& p, cudaStream_t st)
+{
+    return p.pieces > p.splits ? launch_product_t<CG, AMN, BMN, EPI, true>(a, b, o, pre, p, st)
+                               : launch_product_t<CG, AMN, BMN, EPI, false>(a, b, o, pre, p, st);
+}
+
+enum Layout { kKK = 0, kKMN = 1, kMNMN = 2 };  // how A and B are stored
+
+template <int EPI>
+knng_gpu_status launch_any(int cg, Layout lay, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
+                           const CUtensorMap& pre, const ProductParams& p, cudaStream_t st)
+{
+    if constexpr (EPI == kEpiStore) {
+        if (lay == kKMN)
+            return cg == 2 ? launch_product<2, false, true, EPI>(a, b, o, pre, p, st)
+                           : launch_product<1, false, true, EPI>(a, b, o, pre, p, st);
+        if (lay == kMNMN)
+            return cg == 2 ? launch_product<2, true, true, EPI>(a, b, o, pre, p, st)
+                           : launch_product<1, true, true, EPI>(a, b, o, pre, p, st);
+    }
+    return cg == 2 ? launch_product<2, false, false, EPI>(a, b, o, pre, p, st)
+                   : launch_product<1, false, false, EPI>(a, b, o, pre, p, st);
+}
+
+knng_gpu_status operand_maps(const Operand& a, const Operand& b, Layout lay, int in_type, CUtensorMap* ma,
+                             CUtensorMap* mb)
+{
+    KNNG_TRY(make_map(ma, in_type, a.ptr, a.width, a.rows, a.ld, 64, lay == kMNMN ? 64 : 128));
+    return make_map(mb, in_type, b.ptr, b.width, b.rows, b.ld, 64, lay == kKK ? 128 : 64);
+}
+
+int operand_type(int dtype) { return dtype == KNNG_DTYPE_F16 ? kF16 : kBF16; }
+
+ProductParams base_params(const Shape& s, const Plan& q, const Operand& a, const Operand& b, int dtype, int* err)
+{
+    ProductParams p = {};
+    p.m = static_cast<uint32_t>(s.m);
+    p.n = static_cast<uint32_t>(s.n);
+    p.tiles_m = q.tiles_m;
+    p.tiles_n = q.tiles_n;
+    p.splits = q.splits;
+    p.segments = 1;
+    p.items = q.tiles_m * q.tiles_n * q.splits;
+    p.kblocks = q.kblocks;
+    p.piece = q.piece;
+    p.pieces = q.pieces();
+    p.combos = s.combos;
+    p.plane_a = a.plane;
+    p.plane_b = b.plane;
+    p.in_type = operand_type(dtype);
+    p.error = err;
+    p.wait_limit = kSpinLimitCycles;
+    p.alpha = 1.0f;
+    return p;
+}
+
+// What follows a product: the linear epilogue.
+struct Tail {
+    void* out;
+    uint64_t ldo;
+    int out_type;
+    void* pre = nullptr;
+    uint64_t ldp = 0;
+    const void* bias = nullptr;
+    const void* residual = nullptr;
+    uint64_t ldr = 0;
+    int aux_type = KNNG_DTYPE_BF16;
+    int activation = KNNG_ACT_NONE;
+    float alpha = 1.0f;
+    const float* alpha_dev = nullptr;
+};
+
+// D = A B^T through the tail; `part` holds the pieces where the plan splits K.
+knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, const Operand& b, Layout lay, int dtype,
+                              const Tail& t, float* part, int* err, cudaStream_t st)
+{
+    CUtensorMap ma, mb, mo, mp;
+    KNNG_TRY(operand_maps(a, b, lay, operand_type(dtype), &ma, &mb));
+    ProductParams p = base_params(s, q, a, b, dtype, err);
+    if (q.splits > 1) {
+        p.out = part;
+        p.out_type = kF32;
+        p.out_tma = 1;
+        p.split_rows = static_cast<uint32_t>(q.split_rows);
+        KNNG_TRY(make_map(&mo, KNNG_DTYPE_F32, part, q.part_pitch, q.splits * q.split_rows, q.part_pitch, 32, 32));
+        KNNG_TRY(launch_any<kEpiStore>(q.cg, lay, ma, mb, mo, mo, p, st));
+        JoinParams j = {};
+        j.part = part;
+        j.splits = q.splits;
+        j.split_rows = q.split_rows;
+        j.pitch = static_cast<uint32_t>(q.part_pitch);
+        j.m = s.m;
+        j.n = static_cast<uint32_t>(s.n);
+        j.alpha = t.alpha;
+        j.alpha_dev = t.alpha_dev;
+        j.bias = t.bias;
+        j.residual = t.residual;
+        j.ldr = t.ldr;
+        j.aux_type = t.aux_type;
+        j.activation = t.activation;
+        j.out = t.out;
+        j.ldo = t.ldo;
+        j.out_type = t.out_type;
+        j.pre = t.pre;
+        j.ldp = t.ldp;
+        const uint64_t blocks = std::min<uint64_t>(ceil_div(s.m * ceil_div(s.n, 4), 256), 148ull * 16);
+        join_splits_kernel<<<static_cast<uint32_t>(blocks), 256, 0, st>>>(j);
+        KNNG_CUDA(cudaGetLastError());
+        return KNNG_GPU_OK;
+    }
+    p.out = t.out;
+    p.ldo = t.ldo;
+    p.out_type = t.out_type;
+    p.out_tma = tma_rows(t.out, t.ldo, elem_bytes(t.out_type));
+    p.pre = t.pre;
+    p.ldp = t.ldp;
+    p.pre_tma = t.pre && tma_rows(t.pre, t.ldp, elem_bytes(t.aux_type));
+    p.bias = t.bias;
+    p.residual = t.residual;
+    p.ldr = t.ldr;
+    p.aux_type = t.aux_type;
+    p.residual_vec = t.residual && tma_rows(t.residual, t.ldr, elem_bytes(t.aux_type));
+    p.activation = t.activation;
+    p.alpha = t.alpha;
+    p.alpha_dev = t.alpha_dev;
+    mo = ma;
+    mp = ma;
+    if (p.out_tma) KNNG_TRY(make_map(&mo, t.out_type, t.out, s.n, s.m, t.ldo, 128 / elem_bytes(t.out_type), 32));
+    if (p.pre_tma) KNNG_TRY(make_map(&mp, t.aux_type, t.pre, s.n, s.m, t.ldp, 32, 32));
+    return launch_any<kEpiStore>(q.cg, lay, ma, mb, mo, mp, p, st);
+}
+
+// ------------------------------------------------------------------ checks
+constexpr uint64_t kMaxRows = (1ull << 31) - 512;
+constexpr uint64_t kMaxWidth = 1ull << 20;
+
+knng_gpu_status check_matrix(const char* op, const char* name, const void* p, uint64_t rows, uint64_t width,
+                             uint64_t ld, int dtype)
+{
+    if (rows && !p) return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": " + name + " is NULL");
+    if (ld < width)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": row stride of " + name + " (" + std::to_string(ld) +
+                                                   ") must be >= its width (" + std::to_string(width) + ")");
+    if (reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype))
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": " + name + " is not aligned to its elements");
+    return KNNG_GPU_OK;
+}
+
+knng_gpu_status check_sizes(const char* op, uint64_t m, uint64_t k, uint64_t n, int dtype)
+{
+    if (dtype != KNNG_DTYPE_F32 && dtype != KNNG_DTYPE_BF16 && dtype != KNNG_DTYPE_F16)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": unknown dtype " + std::to_string(dtype));
+    if (k == 0) return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": k must be > 0");
+    if (n == 0) return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": n must be > 0");
+    if (m > kMaxRows || n > kMaxRows || k > kMaxWidth)
+        return fail(KNNG_GPU_NOT_SUPPORTED, std::string(op) + ": m and n must be < 2^31 - 512, k <= 2^20");
+    return KNNG_GPU_OK;
+}
+
+// Work items are counted in 32 bits.
+knng_gpu_status check_items(const char* op, const Plan& q)
+{
+    if (uint64_t(q.tiles_m) * q.tiles_n * q.splits >= (1ull << 31))
+        return fail(KNNG_GPU_NOT_SUPPORTED, std::string(op) + ": too many output tiles in one call");
+    return KNNG_GPU_OK;
+}
+
+knng_gpu_status check_workspace(const char* op, const void* ws, uint64_t have, uint64_t need)
+{
+    if (need == 0) return KNNG_GPU_OK;
+    if (!ws || have < need)
+        return fail(KNNG_GPU_WORKSPACE_TOO_SMALL, std::string(op) + ": workspace of " + std::to_string(have) +
+                                                      " bytes, needs " + std::to_string(need));
+    if (reinterpret_cast<uintptr_t>(ws) & 255)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": workspace must be 256-byte aligned");
+    return KNNG_GPU_OK;
+}
+
+// ------------------------------------------------------------------ linear
+// With `need` the bytes of workspace only.
+knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_bytes, cudaStream_t st, uint64_t* need)
+{
+    static const char* const op = "knng::gpu::linear";
+    KNNG_TRY(check_sizes(op, a.m, a.k, a.n, a.dtype));
+    if (a.out_dtype != a.dtype && a.out_dtype != KNNG_DTYPE_F32)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": out_dtype must be dtype or fp32");
+    if (a.activation < KNNG_ACT_NONE || a.activation > KNNG_ACT_SILU)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": unknown activation " + std::to_string(a.activation));
+    if (need) *need = 0;
+    if (a.m == 0) return KNNG_GPU_OK;
+    const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
+    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, a.out_dtype == KNNG_DTYPE_F32};
+    const Plan q = plan_product(s);
+    KNNG_TRY(check_items(op, q));
+    Carver c(ws);
+    uint16_t* xs = needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
+    uint16_t* wst = needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
+    float* part = q.splits > 1 ? c.take<float>(q.part_elems()) : nullptr;
+    if (need) {
+        *need = c.at;
+        return KNNG_GPU_OK;
+    }
+    KNNG_TRY(check_matrix(op, "x", a.x, a.m, a.k, a.ldx, a.dtype));
+    KNNG_TRY(check_matrix(op, "w", a.w, a.n, a.k, a.ldw, a.dtype));
+    KNNG_TRY(check_matrix(op, "out", a.out, a.m, a.n, a.ldo, a.out_dtype));
+    if (a.residual) KNNG_TRY(check_matrix(op, "residual", a.residual, a.m, a.n, a.ldr, a.dtype));
+    if (a.pre) KNNG_TRY(check_matrix(op, "pre", a.pre, a.m, a.n, a.ldp, a.dtype));
+    if (a.bias) KNNG_TRY(check_matrix(op, "bias", a.bias, 1, a.n, a.n, a.dtype));
+    KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
+    int* err;
+    KNNG_TRY(take_error(&err));
+    Operand ox, ow;
+    KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
+    KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+    Tail t{a.out, a.ldo, a.out_dtype};
+    t.pre = a.pre;
+    t.ldp = a.ldp;
+    t.bias = a.bias;
+    t.residual = a.residual;
+    t.ldr = a.ldr;
+    t.aux_type = a.dtype;
+    t.activation = a.activation;
+    return product_store(s, q, ox, ow, kKK, a.dtype, t, part, err, st);
+}
+
+// ------------------------------------------------------------------ linear backward
+knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void* ws, uint64_t ws_bytes,
+                                    cudaStream_t st, uint64_t* need)
+{
+    static const char* const op = "knng::gpu::linear_backward";
+    KNNG_TRY(check_sizes(op, a.m, a.k, a.n, a.dtype));
+    if (a.activation < KNNG_ACT_NONE || a.activation > KNNG_ACT_SILU)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": unknown activation " + std::to_string(a.activation));
+    if (need) *need = 0;
+    const uint32_t e = elem_bytes(a.dtype);
+    if (a.m == 0) {
+        if (need) return KNNG_GPU_OK;
+        if (a.dw) KNNG_CUDA(cudaMemsetAsync(a.dw, 0, a.n * a.k * e, st));
+        if (a.db) KNNG_CUDA(cudaMemsetAsync(a.db, 0, a.n * e, st));
+        return KNNG_GPU_OK;
+    }
+    if (a.activation != KNNG_ACT_NONE && !a.pre)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": pre is NULL with an activation");
+    const bool f32 = a.dtype == KNNG_DTYPE_F32;
+    const uint32_t combos = f32 ? 6 : 1;
+    const Source dy{a.dy, a.m, a.n, a.lddy}, x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
+    const bool slope = a.activation != KNNG_ACT_NONE;
+    const bool products = a.dx || a.dw;
+    // dz lies in the workspace unless it is dy and TMA can read that.
+    const bool make_dz = products && (slope || needs_stage(dy, a.dtype));
+    const Shape sx{a.m, a.k, a.n, combos, f32}, sw{a.n, a.k, a.m, combos, f32};
+    const Plan qx = plan_product(sx), qw = plan_product(sw);
+    KNNG_TRY(check_items(op, qx));
+    KNNG_TRY(check_items(op, qw));
+    const uint64_t pitch = stage_pitch(a.n, a.dtype);
+    const uint32_t gx = static_cast<uint32_t>(ceil_div(pitch, 256));
+    const uint32_t gy = static_cast<uint32_t>(std::max<uint64_t>(
+        1, std::min<uint64_t>({ceil_div(148 * 8, gx), ceil_div(a.m, 8), 65535})));
+    Carver c(ws);
+    uint16_t* dz = make_dz ? c.take<uint16_t>(a.m * pitch * planes_of(a.dtype)) : nullptr;
+    uint16_t* xs = a.dw && needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
+    uint16_t* wst = a.dx && needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
+    float* sums = a.db ? c.take<float>(uint64_t(gy) * a.n) : nullptr;
+    const uint64_t part_elems = std::max(a.dx ? qx.part_elems() : 0, a.dw ? qw.part_elems() : 0);
+    float* part = part_elems ? c.take<float>(part_elems) : nullptr;
+    if (need) {
+        *need = c.at;
+        return KNNG_GPU_OK;
+    }
+    KNNG_TRY(check_matrix(op, "dy", a.dy, a.m, a.n, a.lddy, a.dtype));
+    if (a.dw) KNNG_TRY(check_matrix(op, "x", a.x, a.m, a.k, a.ldx, a.dtype));
+    if (a.dx) KNNG_TRY(check_matrix(op, "w", a.w, a.n, a.k, a.ldw, a.dtype));
+    if (slope) KNNG_TRY(check_matrix(op, "pre", a.pre, a.m, a.n, a.ldp, a.dtype));
+    if (a.dx) KNNG_TRY(check_matrix(op, "dx", a.dx, a.m, a.k, a.k, a.dtype));
+    if (a.dw) KNNG_TRY(check_matrix(op, "dw", a.dw, a.n, a.k, a.k, a.dtype));
+    if (a.db) KNNG_TRY(check_matrix(op, "db", a.db, 1, a.n, a.n, a.dtype));
+    KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
+    int* err;
+    KNNG_TRY(take_error(&err));
+    if (make_dz || a.db) {
+        SlopeParams p = {};
+        p.dy = a.dy;
+        p.lddy = a.lddy;
+        p.pre = slope ? a.pre : nullptr;
+        p.ldp = a.ldp;
+        p.m = a.m;
+        p.n = static_cast<uint32_t>(a.n);
+        p.type = a.dtype;
+        p.activation = a.activation;
+        p.out = dz;
+        p.pitch = static_cast<uint32_t>(pitch);
+        p.planes = planes_of(a.dtype);
+        p.sums = sums;
+        p.vec = tma_rows(a.dy, a.lddy, e) && (!slope || tma_rows(a.pre, a.ldp, e));
+        slope_kernel<<<dim3(gx, gy), 256, 0, st>>>(p);
+        KNNG_CUDA(cudaGetLastError());
+        if (a.db) {
+            join_sums_kernel<<<static_cast<uint32_t>(ceil_div(a.n, 32)), 256, 0, st>>>(
+                sums, gy, static_cast<uint32_t>(a.n), a.db, a.dtype);
+            KNNG_CUDA(cudaGetLastError());
+        }
+    }
+    if (!products) return KNNG_GPU_OK;
+    Operand oz = direct(dy);
+    if (make_dz)
+        oz = Operand{dz, a.m, pitch * planes_of(a.dtype), pitch * planes_of(a.dtype), static_cast<uint32_t>(pitch)};
+    if (a.dx) {
+        Operand ow;
+        KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+        Tail t{a.dx, a.k, a.dtype};
+        KNNG_TRY(product_store(sx, qx, oz, ow, kKMN, a.dtype, t, part, err, st));
+    }
+    if (a.dw) {
+        Operand ox;
+        KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
+        Tail t{a.dw, a.k, a.dtype};
+        KNNG_TRY(product_store(sw, qw, oz, ox, kMNMN, a.dtype, t, part, err, st));
+    }
+    return KNNG_GPU_OK;
+}
+
+// ------------------------------------------------------------------ softmax loss
+knng_gpu_status check_scale(const char* op, float scale)
+{
+    if (!(scale > 0.0f) || !std::isfinite(scale))
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": scale must be finite and > 0");
+    return KNNG_GPU_OK;
+}
+
+knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, uint64_t ws_bytes, cudaStream_t st,
+                                 uint64_t* need)
+{
+    static const char* const op = "knng::gpu::softmax_xent";
+    KNNG_TRY(check_sizes(op, a.m, a.k, a.n, a.dtype));
+    KNNG_TRY(check_scale(op, a.scale));
+    if (need) *need = 0;
+    if (a.m == 0) return KNNG_GPU_OK;
+    const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
+    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, true};
+    // Pairs unless they would leave SMs idle; then the columns are cut so that
+    // (row tile, piece) items fill the units in whole rounds.
+    Plan q = tiles_of(s, 2);
+    if (s.m <= 128 || uint64_t(q.tiles_m) * q.tiles_n < sm_count() / 2) q = tiles_of(s, 1);
+    KNNG_TRY(check_items(op, q));
+    const uint32_t units = sm_count() / q.cg;
+    const uint32_t segments = std::min(q.tiles_n, std::max(1u, static_cast<uint32_t>(ceil_div(units, q.tiles_m))));
+    Carver c(ws);
+    uint16_t* xs = needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
+    uint16_t* wst = needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
+    float2* part = c.take<float2>(2ull * segments * a.m);
+    float* label_dot = c.take<float>(a.m);
+    if (need) {
+        *need = c.at;
+        return KNNG_GPU_OK;
+    }
+    KNNG_TRY(check_matrix(op, "x", a.x, a.m, a.k, a.ldx, a.dtype));
+    KNNG_TRY(check_matrix(op, "w", a.w, a.n, a.k, a.ldw, a.dtype));
+    if (!a.labels || !a.loss || !a.lse) return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": labels, loss or lse is NULL");
+    KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
+    int* err;
+    KNNG_TRY(take_error(&err));
+    Operand ox, ow;
+    KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
+    KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+    CUtensorMap ma, mb;
+    KNNG_TRY(operand_maps(ox, ow, kKK, operand_type(a.dtype), &ma, &mb));
+    ProductParams p = base_params(s, q, ox, ow, a.dtype, err);
+    p.segments = segments;
+    p.items = q.tiles_m * segments;
+    p.scale2 = a.scale * 1.44269504088896f;
+    p.labels = a.labels;
+    p.labels_i64 = a.labels_i64;
+    p.classes = static_cast<uint32_t>(a.n);
+    p.part = part;
+    p.label_dot = label_dot;
+    KNNG_TRY(launch_any<kEpiSoftmax>(q.cg, kKK, ma, mb, ma, ma, p, st));
+    join_softmax_kernel<<<static_cast<uint32_t>(ceil_div(a.m, 8)), 256, 0, st>>>(
+        part, 2 * segments, a.m, label_dot, p.scale2, a.labels, a.labels_i64, static_cast<uint32_t>(a.n), a.loss, a.lse);
+    KNNG_CUDA(cudaGetLastError());
+    return KNNG_GPU_OK;
+}
+
+// ------------------------------------------------------------------ softmax loss, gradient
+// Bytes of one piece's g: a share of the 126 MB L2, so that the two products
+// that read it find it there.
+constexpr uint64_t kPieceBytes = 64ull << 20;
+
+knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_args& a, void* ws, uint64_t ws_bytes,
+                                          cudaStream_t st, uint64_t* need)
+{
+    static const char* const op = "knng::gpu::softmax_xent_backward";
+    KNNG_TRY(check_sizes(op, a.m, a.k, a.n, a.dtype));
+    KNNG_TRY(check_scale(op, a.scale));
+    if (need) *need = 0;
+    const uint32_t e = elem_bytes(a.dtype);
+    if (a.m == 0) {
+        if (need || !a.dw) return KNNG_GPU_OK;
+        KNNG_CUDA(cudaMemsetAsync(a.dw, 0, a.n * a.k * e, st));
+        return KNNG_GPU_OK;
+    }
+    const uint32_t planes = planes_of(a.dtype);
+    const uint32_t combos = planes == 3 ? 6 : 1;
+    const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
+    // Columns per piece: whole tiles, at least 2048 so that each product fills the GPU, all pieces alike.
+    const uint64_t want = std::max<uint64_t>(2048, kPieceBytes / (2 * planes * a.m) / 256 * 256);
+    const uint64_t pieces = ceil_div(a.n, want);
+    const uint64_t width = up(ceil_div(a.n, pieces), 256);
+    const uint64_t gpitch = up(std::min(width, a.n), 64);
+    const bool f32 = planes == 3;
+    const Shape sg{a.m, std::min(width, a.n), a.k, combos, f32};
+    const Shape sx{a.m, a.k, std::min(width, a.n), combos, f32};
+    const Plan qx = plan_product(sx);
+    const uint64_t xpart_rows = qx.split_rows, xpart_pitch = qx.part_pitch;
+    const auto dw_shape = [&](uint64_t cols) { return Shape{cols, a.k, a.m, combos, f32}; };
+    const uint64_t last = a.n - (ceil_div(a.n, width) - 1) * width;
+    const Plan qw0 = plan_product(dw_shape(std::min(width, a.n))), qw1 = plan_product(dw_shape(last));
+    for (const Plan& q : {tiles_of(sg, 1), qx, qw0, qw1}) KNNG_TRY(check_items(op, q));
+    Carver c(ws);
+    uint16_t* xs = c.take<uint16_t>(stage_elems(x, a.dtype));
+    uint16_t* wst = needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
+    float* coef = c.take<float>(a.m);
+    float* lse2 = c.take<float>(a.m);
+    float* cmax = c.take<float>(1);
+    uint16_t* g = c.take<uint16_t>(a.m * gpitch * planes);
+    float* xpart = a.dx ? c.take<float>(qx.splits * xpart_rows * xpart_pitch) : nullptr;
+    const uint64_t wpart_elems = a.dw ? std::max(qw0.part_elems(), qw1.part_elems()) : 0;
+    float* wpart = wpart_elems ? c.take<float>(wpart_elems) : nullptr;
+    if (need) {
+        *need = c.at;
+        return KNNG_GPU_OK;
+    }
+    KNNG_TRY(check_matrix(op, "x", a.x, a.m, a.k, a.ldx, a.dtype));
+    KNNG_TRY(check_matrix(op, "w", a.w, a.n, a.k, a.ldw, a.dtype));
+    if (a.dx) KNNG_TRY(check_matrix(op, "dx", a.dx, a.m, a.k, a.k, a.dtype));
+    if (a.dw) KNNG_TRY(check_matrix(op, "dw", a.dw, a.n, a.k, a.k, a.dtype));
+    if (!a.labels || !a.dloss || !a.lse)
+        return fail(KNNG_GPU_INVALID_ARGUMENT, std::string(op) + ": labels, dloss or lse is NULL");
+    KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
+    if (!a.dx && !a.dw) return KNNG_GPU_OK;
+    int* err;
+    KNNG_TRY(take_error(&err));
+    const RowLabels labels{a.labels, a.labels_i64, static_cast<uint32_t>(a.n)};
+    Operand ox, ow;
+    KNNG_TRY(stage(x, a.dtype, xs, &ox, st, labels));
+    KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+    KNNG_CUDA(cudaMemsetAsync(cmax, 0, 4, st));
+    grad_rows_kernel<<<static_cast<uint32_t>(std::min<uint64_t>(ceil_div(a.m, 256), 148)), 256, 0, st>>>(
+        a.dloss, a.lse, a.m, a.scale, a.labels, a.labels_i64, static_cast<uint32_t>(a.n), coef, lse2,
+        reinterpret_cast<uint32_t*>(cmax));
+    KNNG_CUDA(cudaGetLastError());
+    // fp16 holds 2^14 g / max |dloss scale|: |g| <= 1 there, and the smallest
+    // normal value 6e-5 then stands for 4e-9 instead of losing every p below it.
+    const float gscale = a.dtype == KNNG_DTYPE_F16 ? 16384.0f : 1.0f;
+    for (uint64_t c0 = 0; c0 < a.n; c0 += width) {
+        const uint64_t cols = std::min(width, a.n - c0);
+        const Operand wp{static_cast<const uint16_t*>(ow.ptr) + c0 * ow.ld, cols, ow.width, ow.ld, ow.plane};
+        const Shape s1{a.m, cols, a.k, combos, f32};
+        Plan q1 = tiles_of(s1, 2);
+        if (uint64_t(q1.tiles_m) * q1.tiles_n * 2 < sm_count() * 3ull / 4) q1 = tiles_of(s1, 1);
+        CUtensorMap ma, mb, mo;
+        KNNG_TRY(operand_maps(ox, wp, kKK, operand_type(a.dtype), &ma, &mb));
+        ProductParams p = base_params(s1, q1, ox, wp, a.dtype, err);
+        p.scale2 = a.scale * 1.44269504088896f;
+        p.labels = a.labels;
+        p.labels_i64 = a.labels_i64;
+        p.classes = static_cast<uint32_t>(a.n);
+        p.class0 = static_cast<uint32_t>(c0);
+        p.lse2 = lse2;
+        p.coef = coef;
+        p.alpha_dev = cmax;
+        p.grad_scale = gscale;
+        p.grad_planes = planes;
+        p.grad_pitch = static_cast<uint32_t>(gpitch);
+        const uint64_t gld = gpitch * planes;
+        const uint64_t gwidth = planes == 1 ? cols : gld;
+        KNNG_TRY(make_map(&mo, operand_type(a.dtype), g, gwidth, a.m, gld, 64, 32));
+        KNNG_TRY(launch_any<kEpiGrad>(q1.cg, kKK, ma, mb, mo, mo, p, st));
+        const Operand og{g, a.m, gwidth, gld, static_cast<uint32_t>(gpitch)};
+        if (a.dw) {
+            const Shape sw = dw_shape(cols);
+            const Plan qw = plan_product(sw);
+            Tail t{static_cast<uint8_t*>(a.dw) + c0 * a.k * e, a.k, a.dtype};
+            t.alpha = 1.0f / gscale;
+            t.alpha_dev = cmax;
+            KNNG_TRY(product_store(sw, qw, og, ox, kMNMN, a.dtype, t, wpart, err, st));
+        }
+        if (a.dx) {
+            // Pieces add up in fp32: the first one stores, the others add.
+            const Shape sp{a.m, a.k, cols, combos, f32};
+            Plan qp = qx;
+            qp.kblocks = static_cast<uint32_t>(ceil_div(cols, 64));
+            qp.splits = std::min(qx.splits, qp.pieces());
+            CUtensorMap mga, mwb, mx;
+            KNNG_TRY(operand_maps(og, wp, kKMN, operand_type(a.dtype), &mga, &mwb));
+            ProductParams px = base_params(sp, qp, og, wp, a.dtype, err);
+            px.out = xpart;
+            px.out_type = kF32;
+            px.out_tma = 1;
+            px.accumulate = c0 > 0;
+            px.split_rows = static_cast<uint32_t>(xpart_rows);
+            KNNG_TRY(make_map(&mx, KNNG_DTYPE_F32, xpart, xpart_pitch, qx.splits * xpart_rows, xpart_pitch, 32, 32));
+            KNNG_TRY(launch_any<kEpiStore>(qp.cg, kKMN, mga, mwb, mx, mx, px, st));
+        }
+    }
+    if (a.dx) {
+        JoinParams j = {};
+        j.part = xpart;
+        j.splits = qx.splits;
+        j.split_rows = xpart_rows;
+        j.pitch = static_cast<uint32_t>(xpart_pitch);
+        j.m = a.m;
+        j.n = static_cast<uint32_t>(a.k);
+        j.alpha = 1.0f / gscale;
+        j.alpha_dev = cmax;
+        j.out = a.dx;
+        j.ldo = a.k;
+        j.out_type = a.dtype;
+        j.labels = a.labels;
+        j.labels_i64 = a.labels_i64;
+        j.classes = static_cast<uint32_t>(a.n);
+        const uint64_t blocks = std::min<uint64_t>(ceil_div(a.m * ceil_div(a.k, 4), 256), 148ull * 16);
+        join_splits_kernel<<<static_cast<uint32_t>(blocks), 256, 0, st>>>(j);
+        KNNG_CUDA(cudaGetLastError());
+    }
+    return KNNG_GPU_OK;
+}
+
+// No exception leaves a C entry point.
+template <class F>
+knng_gpu_status guarded(F&& f)
+{
+    try {
+        clear_last_error();
+        return f();
+    } catch (const std::bad_alloc&) {
+        return KNNG_GPU_OUT_OF_MEMORY;
+    } catch (...) {
+        return KNNG_GPU_CUDA_ERROR;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+#define KNNG_LEARN_ENTRY(name)                                                                              \
+    uint64_t knng_gpu_##name##_workspace_bytes(const knng_gpu_##name##_args* a)                             \
+    {                                                                                                       \
+        uint64_t need = 0;                                                                                  \
+        if (!a) return 0;                                                                                   \
+        const knng_gpu_status s = guarded([&] { return name##_run(*a, nullptr, 0, nullptr, &need); });      \
+        return s == KNNG_GPU_OK ? need : 0;                                                                 \
+    }                                                                                                       \
+    knng_gpu_status knng_gpu_##name(const knng_gpu_##name##_args* a, void* d_workspace,                     \
+                                    uint64_t workspace_bytes, void* stream)                                 \
+    {                                                                                                       \
+        return guarded([&] {                                                                                \
+            if (!a) return fail(KNNG_GPU_INVALID_ARGUMENT, "knng::gpu::" #name ": args is NULL");           \
+            return name##_run(*a, d_workspace, workspace_bytes, static_cast<cudaStream_t>(stream), nullptr); \
+        });                                                                                                 \
+    }
+
+KNNG_LEARN_ENTRY(linear)
+KNNG_LEARN_ENTRY(linear_backward)
+KNNG_LEARN_ENTRY(softmax_xent)
+KNNG_LEARN_ENTRY(softmax_xent_backward)
+
+}  // extern "C"

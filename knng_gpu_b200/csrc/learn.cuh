@@ -1,0 +1,329 @@
+// learn.cuh -- the kernels around the tensor-core product of product.cuh:
+// staging of rows that TMA cannot read (odd strides, fp32), the joins of split
+// products and of softmax pieces, dz = dy act'(pre) with its column sums. All
+// are bound by HBM (one read, one write) or, on small calls, by launch latency.
+#pragma once
+#include "product.cuh"
+
+namespace knng_b200 {
+
+// Rows as 16-bit operands: `planes` = 1 copies 16-bit rows to a pitch that TMA
+// can read, 3 splits fp32 values into bf16 parts x = h + m + l (each rounded to
+// nearest from what is left; a finite value whose rounding would overflow is
+// truncated). Columns past k are zeros. Rows without a label are zeros when
+// labels are given. One thread per 8 columns.
+template <int PLANES>
+__global__ void __launch_bounds__(256) stage_rows_kernel(const void* __restrict__ x, uint64_t rows, uint32_t k,
+                                                         uint64_t ld, uint16_t* __restrict__ out, uint32_t pitch,
+                                                         const void* labels, int labels_i64, uint32_t classes)
+{
+    const uint32_t groups = pitch / 8;
+    const uint64_t total = rows * groups;
+    for (uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+        const uint64_t r = i / groups;
+        const uint32_t c0 = static_cast<uint32_t>(i - r * groups) * 8;
+        const bool keep = !labels || load_label(labels, labels_i64, r, classes) >= 0;
+        if constexpr (PLANES == 1) {
+            const uint16_t* src = static_cast<const uint16_t*>(x) + r * ld;
+            uint32_t w[4];
+            if (keep && c0 + 8 <= k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
+                const uint4 q = *reinterpret_cast<const uint4*>(src + c0);
+                w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a = keep && c0 + 2 * j < k ? src[c0 + 2 * j] : 0u;
+                    const uint32_t b = keep && c0 + 2 * j + 1 < k ? src[c0 + 2 * j + 1] : 0u;
+                    w[j] = a | (b << 16);
+                }
+            }
+            *reinterpret_cast<uint4*>(out + r * pitch + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            const float* src = static_cast<const float*>(x) + r * ld;
+            float v[8];
+            if (keep && c0 + 8 <= k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
+                const float4 a = *reinterpret_cast<const float4*>(src + c0);
+                const float4 b = *reinterpret_cast<const float4*>(src + c0 + 4);
+                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+                v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = keep && c0 + j < k ? src[c0 + j] : 0.0f;
+            }
+            uint16_t* dst = out + r * (3ull * pitch) + c0;
+#pragma unroll
+            for (int plane = 0; plane < 3; ++plane) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h2 = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float& f = v[2 * j + h];
+                        __nv_bfloat16 b = __float2bfloat16_rn(f);
+                        if (isinf(__bfloat162float(b)) && !isinf(f)) b = __float2bfloat16_rz(f);
+                        uint16_t bits;
+                        memcpy(&bits, &b, 2);
+                        h2 |= static_cast<uint32_t>(bits) << (16 * h);
+                        f -= __bfloat162float(b);
+                    }
+                    w[j] = h2;
+                }
+                *reinterpret_cast<uint4*>(dst + uint64_t(plane) * pitch) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+struct JoinParams {
+    const float* part;      // [splits][split_rows][pitch]
+    uint32_t splits;
+    uint64_t split_rows;
+    uint32_t pitch;         // multiple of 4
+    uint64_t m;
+    uint32_t n;
+    float alpha;
+    const float* alpha_dev;
+    const void* bias;
+    const void* residual;
+    uint64_t ldr;
+    int aux_type;
+    int activation;
+    void* out;
+    uint64_t ldo;
+    int out_type;
+    void* pre;
+    uint64_t ldp;
+    const void* labels;     // rows without a label become zeros
+    int labels_i64;
+    uint32_t classes;
+};
+
+// The pieces of a split product, summed in order, and the linear epilogue.
+__global__ void __launch_bounds__(256) join_splits_kernel(const JoinParams p)
+{
+    const uint32_t groups = (p.n + 3) / 4;
+    const uint64_t total = p.m * groups;
+    const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
+    for (uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+        const uint64_t r = i / groups;
+        const uint32_t c = static_cast<uint32_t>(i - r * groups) * 4;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (!p.labels || load_label(p.labels, p.labels_i64, r, p.classes) >= 0) {
+            for (uint32_t s = 0; s < p.splits; ++s) {
+                const float4 q = *reinterpret_cast<const float4*>(p.part + (s * p.split_rows + r) * p.pitch + c);
+                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] *= alpha;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j >= p.n) break;
+            float z = v[j];
+            if (p.bias) z += load_elem(p.bias, c + j, p.aux_type);
+            if (p.pre) store_elem(p.pre, r * p.ldp + c + j, z, p.aux_type);
+            z = act_dyn(z, p.activation);
+            if (p.residual) z += load_elem(p.residual, r * p.ldr + c + j, p.aux_type);
+            store_elem(p.out, r * p.ldo + c + j, z, p.out_type);
+        }
+    }
+}
+
+// Joins a row's softmax pieces, which leave the label's own term out: with M
+// the largest other score, S = sum of 2^(score - M) over the others and y the
+// label's score, in base 2,
+//   loss = log(1 + S 2^(M - y)), lse = y ln 2 + loss        where y >= M,
+//   loss = (M - y) ln 2 + log(S + 2^(y - M)), lse likewise  where it is not.
+// So the small loss of a well placed row keeps its digits. Without a label
+// lse = M ln 2 + log S. One warp per row.
+__global__ void __launch_bounds__(256) join_softmax_kernel(const float2* __restrict__ part, uint32_t pieces,
+                                                           uint64_t m, const float* __restrict__ label_dot,
+                                                           float scale2, const void* labels, int labels_i64,
+                                                           uint32_t classes, float* __restrict__ loss,
+                                                           float* __restrict__ lse)
+{
+    const uint64_t r = blockIdx.x * uint64_t(8) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (r >= m) return;
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t s = lane; s < pieces; s += 32) {
+        const float2 q = part[uint64_t(s) * m + r];
+        const float now = fmaxf(top, q.x);
+        const float base = now == -INFINITY ? 0.0f : now;
+        sum = sum * exp2_approx(top - base) + q.y * exp2_approx(q.x - base);
+        top = now;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const float t2 = __shfl_xor_sync(~0u, top, o), s2 = __shfl_xor_sync(~0u, sum, o);
+        const float now = fmaxf(top, t2);
+        const float base = now == -INFINITY ? 0.0f : now;
+        sum = sum * exp2_approx(top - base) + s2 * exp2_approx(t2 - base);
+        top = now;
+    }
+    if (lane == 0) {
+        const bool has = load_label(labels, labels_i64, r, classes) >= 0;
+        if (!has) {
+            lse[r] = top == -INFINITY ? top : fmaf(top, 0.69314718f, logf(sum));
+            loss[r] = 0.0f;
+        } else {
+            const float y = label_dot[r] * scale2;
+            if (!(y < top)) {  // also a NaN score
+                const float others = sum == 0.0f ? y - y : log1pf(sum * exp2_approx(top - y));
+                loss[r] = others;
+                lse[r] = y == -INFINITY ? y : fmaf(y, 0.69314718f, others);
+            } else {
+                const float tail = logf(sum + exp2_approx(y - top));
+                loss[r] = fmaf(top - y, 0.69314718f, tail);
+                lse[r] = fmaf(top, 0.69314718f, tail);
+            }
+        }
+    }
+}
+
+// Per row of the gradient: coef = dloss scale and lse in base 2 (both 0 for a
+// row without a label), and the largest finite |coef| as float bits (a maximum
+// does not depend on the order of the atomics).
+__global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict__ dloss, const float* __restrict__ lse,
+                                                        uint64_t m, float scale, const void* labels, int labels_i64,
+                                                        uint32_t classes, float* __restrict__ coef,
+                                                        float* __restrict__ lse2, uint32_t* cmax)
+{
+    float big = 0.0f;
+    for (uint64_t r = blockIdx.x * uint64_t(256) + threadIdx.x; r < m; r += uint64_t(gridDim.x) * 256) {
+        const bool has = load_label(labels, labels_i64, r, classes) >= 0;
+        const float c = has ? dloss[r] * scale : 0.0f;
+        coef[r] = c;
+        lse2[r] = has ? lse[r] * 1.44269504f : 0.0f;
+        if (isfinite(c)) big = fmaxf(big, fabsf(c));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
+    if ((threadIdx.x & 31) == 0 && big > 0.0f) atomicMax(cmax, __float_as_uint(big));
+}
+
+struct SlopeParams {
+    const void* dy;
+    uint64_t lddy;
+    const void* pre;      // may be NULL: dz = dy
+    uint64_t ldp;
+    uint64_t m;
+    uint32_t n;
+    int type;
+    int activation;
+    uint16_t* out;        // dz as 16-bit operands (may be NULL: column sums only)
+    uint32_t pitch;       // columns of a plane of out
+    uint32_t planes;
+    float* sums;          // [gridDim.y][n] column sums (may be NULL)
+    int vec;              // rows of dy and pre allow 16-byte loads
+};
+
+__device__ __forceinline__ void load8(const void* p, uint64_t at, int type, uint32_t left, bool vec, float* v)
+{
+    if (vec && left >= 8) {
+        if (type == kF32) {
+            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+            const float4 a = q[0], b = q[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = unpack2(w[j], type);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < static_cast<int>(left) ? load_elem(p, at + j, type) : 0.0f;
+    }
+}
+
+// dz = dy act'(pre), rounded to the operands' type, and its column sums (of
+// the unrounded values). A block takes 256 columns (8 per lane) and a range of
+// rows; its 8 warps take every eighth row and add up their sums in order.
+__global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
+{
+    __shared__ float total[8][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t c0 = blockIdx.x * 256 + lane * 8;
+    const uint64_t r0 = p.m * blockIdx.y / gridDim.y, r1 = p.m * (blockIdx.y + 1) / gridDim.y;
+    const uint32_t left = c0 < p.n ? p.n - c0 : 0;
+    float acc[8] = {};
+    for (uint64_t r = r0 + warp; r < r1; r += 8) {
+        float v[8] = {};
+        if (left) {
+            load8(p.dy, r * p.lddy + c0, p.type, left, p.vec, v);
+            if (p.pre) {
+                float z[8];
+                load8(p.pre, r * p.ldp + c0, p.type, left, p.vec, z);
+                const uint32_t have = left < 8 ? left : 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (j >= static_cast<int>(have)) break;
+                    switch (p.activation) {
+                        case kActRelu: v[j] *= slope_f<kActRelu>(z[j]); break;
+                        case kActGelu: v[j] *= slope_f<kActGelu>(z[j]); break;
+                        case kActGeluTanh: v[j] *= slope_f<kActGeluTanh>(z[j]); break;
+                        case kActSilu: v[j] *= slope_f<kActSilu>(z[j]); break;
+                        default: break;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += v[j];
+        }
+        if (p.out && c0 < p.pitch) {
+            uint16_t* dst = p.out + r * (uint64_t(p.pitch) * p.planes) + c0;
+            for (uint32_t plane = 0; plane < p.planes; ++plane) {
+                uint32_t w[4];
+                const int type = p.type == kF16 ? kF16 : kBF16;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = pack2(v[2 * j], v[2 * j + 1], type);
+                    const float2 f = unpack2(w[j], type);
+                    v[2 * j] -= f.x;
+                    v[2 * j + 1] -= f.y;
+                }
+                *reinterpret_cast<uint4*>(dst + plane * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    if (p.sums) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) total[warp][lane * 8 + j] = acc[j];
+        __syncthreads();
+        const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+        if (c < p.n) {
+            float s = 0.0f;
+            for (int w = 0; w < 8; ++w) s += total[w][threadIdx.x];
+            p.sums[uint64_t(blockIdx.y) * p.n + c] = s;
+        }
+    }
+}
+
+// Column sums of [rows][n] partial sums: 32 columns per block, 8 row groups
+// added in order.
+__global__ void __launch_bounds__(256) join_sums_kernel(const float* __restrict__ sums, uint32_t rows, uint32_t n,
+                                                        void* out, int type)
+{
+    __shared__ float part[8][32];
+    const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t c = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (c < n)
+        for (uint32_t r = g; r < rows; r += 8) s += sums[uint64_t(r) * n + c];
+    part[g][lane] = s;
+    __syncthreads();
+    if (g == 0 && c < n) {
+        float t = 0.0f;
+        for (int i = 0; i < 8; ++i) t += part[i][lane];
+        store_elem(out, c, t, type);
+    }
+}
+
+}  // namespace knng_b200

@@ -1,0 +1,908 @@
+// product.cuh -- D = A B^T on the tensor cores with a fused epilogue: the one
+// kernel behind the linear layer, the softmax loss over inner products and
+// their gradients.
+//
+//   A is m x K, B is n x K. Either may lie in memory with K contiguous
+//   ("K-major": rows of the operand) or with m / n contiguous ("MN-major": the
+//   operand is the transpose of what is stored), so x w^T, dz w and dz^T x all
+//   read the caller's rows as they lie, without a transposed copy.
+//
+// Operands are bf16 or fp16 with fp32 accumulation in TMEM. fp32 operands come
+// as three bf16 planes (x = h + m + l, each the rounding of what the ones
+// before left) and the product is the six plane products down to 2^-18 of the
+// leading one, summed smallest first into the same accumulator; the three that
+// are left out are below 2^-26 of it.
+//
+// Tile and roles. CG = 2: a CTA pair computes 256 x 256 with
+// tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and 128 of B per
+// 64-wide K block, half of what two single-CTA tiles would read from L2.
+// CG = 1: 128 x 128 by one CTA, for products with too few tiles to fill the
+// GPU with pairs. Per CTA:
+//   warp 0      TMA producer, kStages-deep ring of 32 KiB stages
+//   warp 1      TMEM allocation; UMMA issue (leader CTA, one lane)
+//   warps 2-3   idle
+//   warps 4-11  epilogue: thread = one accumulator row, the two halves of the
+//               warps take the two halves of the columns. Two accumulator
+//               buffers in TMEM: the epilogue of a tile runs under the MMAs of
+//               the next one.
+// Outputs leave through 4 KiB shared-memory boxes per warp and TMA stores
+// (reduce-adds where a call accumulates), or by coalesced element stores where
+// the output rows are not 16-byte aligned.
+//
+// Every wait is bounded: a role that gives up reports through *p.error (host
+// memory), raises the abort flag of its CTA or pair, and all roles unwind.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace knng_b200 {
+
+constexpr int kPkThreads = 384;    // 4 + 8 warps
+constexpr int kPkEpiWarps = 8;
+constexpr int kPkStages = 5;
+constexpr int kPkStageBytes = 32768;  // 128 x 64 of A and of B, 2 bytes each
+constexpr int kPkBox = 4096;          // staging box: 32 rows x 128 bytes
+constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkEpiWarps * 2 * kPkBox + 512 + 1024;
+
+enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+enum Epilogue : int { kEpiStore = 0, kEpiSoftmax = 1, kEpiGrad = 2 };
+
+struct ProductParams {
+    uint32_t m, n;                 // rows and columns of D
+    uint32_t tiles_m, tiles_n;
+    uint32_t splits;               // store: pieces of the K loop, each to its own rows of the output map
+    uint32_t segments;             // softmax: pieces of the columns per row tile
+    uint32_t items;                // work items = tiles_m * tiles_n * splits, or tiles_m * segments
+    uint32_t kblocks;              // 64-wide K blocks of one plane
+    uint32_t piece;                // K blocks (of every plane product) summed in TMEM before they leave it
+    uint32_t pieces;               // ceil(kblocks / piece)
+    uint32_t combos;               // 1, or 6 plane products of split fp32 operands
+    uint32_t plane_a, plane_b;     // columns from one plane to the next in the stored matrices
+    int in_type;                   // kBF16 or kF16
+    int* error;
+    long long wait_limit;
+    // store
+    int out_type;                  // ElemType
+    int out_tma, pre_tma;          // TMA store possible; otherwise element stores through out / pre
+    int accumulate;                // fp32 output: add to what is there
+    void *out, *pre;
+    uint64_t ldo, ldp;
+    uint32_t split_rows;           // rows between the outputs of two splits
+    const void* bias;              // of type aux_type
+    const void* residual;
+    uint64_t ldr;
+    int aux_type;
+    int residual_vec;              // residual rows allow 16-byte loads
+    int activation;
+    float alpha;                   // D is scaled by alpha * *alpha_dev
+    const float* alpha_dev;
+    // softmax and gradient
+    float scale2;                  // scale * log2(e)
+    const void* labels;            // class of each row, int64 or int32; outside [0, classes) where it has none
+    int labels_i64;
+    uint32_t classes;
+    uint32_t class0;               // class of column 0
+    float2* part;                  // softmax: (max, sum) of row r, piece s, column half h at [(2 s + h) * m + r]
+    float* label_dot;              // softmax: x_r . w_label
+    const float* lse2;             // gradient: lse * log2(e)
+    const float* coef;             // gradient: dloss * scale / cmax, 0 for a row without label
+    float grad_scale;              // gradient: power of two on the stored values
+    uint32_t grad_planes, grad_pitch;
+};
+
+// ---------------------------------------------------------------- PTX of this kernel
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Descriptor of an MN-major operand staged as blocks of 64 (MN) x 64 (K): rows
+// of 128 bytes along MN, one per K index, 128-byte swizzle. Eight K rows are
+// 1024 bytes apart (stride offset), the next 64 MN values 8 KiB (leading
+// offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr)
+{
+    uint64_t desc = 0;
+    desc |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    desc |= static_cast<uint64_t>(8192u >> 4) << 16;
+    desc |= static_cast<uint64_t>(1024u >> 4) << 32;
+    desc |= static_cast<uint64_t>(1u) << 46;
+    desc |= static_cast<uint64_t>(2u) << 61;
+    return desc;
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem, int32_t x, int32_t y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_u32(smem))
+                 : "memory");
+}
+
+__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, const void* smem, int32_t x, int32_t y)
+{
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_u32(smem))
+                 : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read()
+{
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---------------------------------------------------------------- elementwise pieces
+__device__ __forceinline__ uint32_t pack2(float a, float b, int type)
+{
+    uint32_t r;
+    if (type == kBF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        memcpy(&r, &v, 4);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        memcpy(&r, &v, 4);
+    }
+    return r;
+}
+
+__device__ __forceinline__ float load_elem(const void* p, uint64_t i, int type)
+{
+    if (type == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    if (type == kF16) return __half2float(static_cast<const __half*>(p)[i]);
+    return static_cast<const float*>(p)[i];
+}
+
+__device__ __forceinline__ void store_elem(void* p, uint64_t i, float v, int type)
+{
+    if (type == kBF16)
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else if (type == kF16)
+        static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else
+        static_cast<float*>(p)[i] = v;
+}
+
+// Two 16-bit values of a word as floats.
+__device__ __forceinline__ float2 unpack2(uint32_t w, int type)
+{
+    if (type == kBF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+}
+
+// sigmoid(v) = 1 / (1 + e^-v); e^-v overflows to +inf for very negative v,
+// where the quotient is 0 as it should be.
+__device__ __forceinline__ float sigmoid_f(float v) { return 1.0f / (1.0f + exp2_approx(-1.44269504f * v)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_f(float z)
+{
+    if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
+    if constexpr (ACT == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    // 0.5 (1 + tanh u) = sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3).
+    if constexpr (ACT == kActGeluTanh) return z * sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
+    if constexpr (ACT == kActSilu) return z * sigmoid_f(z);
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float slope_f(float z)
+{
+    if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (ACT == kActGelu)
+        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * exp2_approx(-0.72134752f * z * z);
+    if constexpr (ACT == kActGeluTanh) {
+        const float s = sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
+        return s + z * s * (1.0f - s) * 1.59576912f * (1.0f + 0.134145f * z * z);
+    }
+    if constexpr (ACT == kActSilu) {
+        const float s = sigmoid_f(z);
+        return s * (1.0f + z * (1.0f - s));
+    }
+    return 1.0f;
+}
+
+// One value of the linear epilogue (shared with the join of split products).
+__device__ __forceinline__ float act_dyn(float z, int act)
+{
+    switch (act) {
+        case kActRelu: return act_f<kActRelu>(z);
+        case kActGelu: return act_f<kActGelu>(z);
+        case kActGeluTanh: return act_f<kActGeluTanh>(z);
+        case kActSilu: return act_f<kActSilu>(z);
+        default: return z;
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_all(float* v)
+{
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_f<ACT>(v[i]);
+}
+
+// The A / B plane of plane product c, smallest products first:
+// l h, h l, m m, m h, h m, h h.
+__device__ __forceinline__ uint32_t combo_a(uint32_t c, uint32_t combos)
+{
+    return combos == 1 ? 0u : (0x001102u >> (4 * c)) & 3u;  // 2,0,1,1,0,0
+}
+__device__ __forceinline__ uint32_t combo_b(uint32_t c, uint32_t combos)
+{
+    return combos == 1 ? 0u : (0x010120u >> (4 * c)) & 3u;  // 0,2,1,0,1,0
+}
+
+// Class of a row, -1 where it has none.
+__device__ __forceinline__ int32_t load_label(const void* labels, int i64, uint64_t row, uint32_t classes)
+{
+    const int64_t y = i64 ? static_cast<const int64_t*>(labels)[row]
+                          : static_cast<int64_t>(static_cast<const int32_t*>(labels)[row]);
+    return y >= 0 && y < static_cast<int64_t>(classes) ? static_cast<int32_t>(y) : -1;
+}
+
+// ---------------------------------------------------------------- schedule
+struct Item {
+    uint32_t tm, n0, n1, p0, p1, split, segment;  // row tile, column tiles, K pieces
+};
+
+template <int EPI>
+__device__ __forceinline__ Item decode_item(const ProductParams& p, uint32_t i)
+{
+    Item t;
+    if constexpr (EPI == kEpiSoftmax) {
+        // Items next to each other walk the same columns for different row
+        // tiles, so B is read from HBM once.
+        t.segment = i / p.tiles_m;
+        t.tm = i % p.tiles_m;
+        t.n0 = static_cast<uint32_t>(uint64_t(t.segment) * p.tiles_n / p.segments);
+        t.n1 = static_cast<uint32_t>(uint64_t(t.segment + 1) * p.tiles_n / p.segments);
+        t.split = 0;
+        t.p0 = 0;
+        t.p1 = p.pieces;
+    } else {
+        // Bands of 8 row tiles, walked column tile by column tile: the units
+        // that run together share A and B tiles in L2.
+        const uint32_t tiles = p.tiles_m * p.tiles_n;
+        t.split = i / tiles;
+        const uint32_t r = i % tiles;
+        const uint32_t band = r / (8 * p.tiles_n);
+        const uint32_t rows = min(8u, p.tiles_m - band * 8);
+        const uint32_t q = r - band * 8 * p.tiles_n;
+        t.tm = band * 8 + q % rows;
+        t.n0 = q / rows;
+        t.n1 = t.n0 + 1;
+        t.segment = 0;
+        t.p0 = static_cast<uint32_t>(uint64_t(t.split) * p.pieces / p.splits);
+        t.p1 = static_cast<uint32_t>(uint64_t(t.split + 1) * p.pieces / p.splits);
+    }
+    return t;
+}
+
+// ---------------------------------------------------------------- kernel
+// LONG: an item may have several K pieces, whose sums are added in registers.
+template <int CG, bool AMN, bool BMN, int EPI, bool LONG>
+__global__ void __launch_bounds__(kPkThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
+                   const ProductParams p)
+{
+    constexpr int BN = 128 * CG;           // columns of a tile
+    constexpr uint32_t kTmemCols = 2 * BN;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* stage_base = smem;
+    uint8_t* boxes = smem + kPkStages * kPkStageBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(boxes + kPkEpiWarps * 2 * kPkBox);
+    uint64_t* full = bars;        // [kPkStages] leader: bytes of both CTAs landed
+    uint64_t* empty = bars + 8;   // [kPkStages] both: MMAs that read the stage are done
+    uint64_t* tfull = bars + 16;  // [2] both: accumulator ready
+    uint64_t* tempty = bars + 18; // [2] leader: accumulator read by the epilogue warps of both CTAs
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 21);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t cta = CG == 2 ? (cluster_ctarank() & 1u) : 0u;
+    const bool leader = cta == 0;
+    const uint32_t unit = blockIdx.x / CG;
+    const uint32_t units = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPkStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], CG * kPkEpiWarps);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&map_a);
+        prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) {
+        if constexpr (CG == 2)
+            tmem_alloc_pair(tmem_slot, kTmemCols);
+        else
+            tmem_alloc(tmem_slot, kTmemCols);
+    }
+    tc_fence_before();
+    if constexpr (CG == 2)
+        cluster_sync_all();
+    else
+        __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    auto abort_all = [&]() {
+        *p.error = 1;
+        __threadfence_system();
+        *abort_flag = 1;
+        if constexpr (CG == 2) st_cluster_u32(mapa_shared(smem_u32(const_cast<int*>(abort_flag)), cta ^ 1u), 1u);
+    };
+
+    // Registers: 168 a thread at launch; the first warpgroup gives up 112 of
+    // them, the two of the epilogue take 56 each (56 + 2 * 224 = 3 * 168).
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (lane == 0) {
+            const uint32_t full_leader = CG == 2 ? mapa_shared(smem_u32(full), 0u) : 0u;
+            uint32_t stage = 0, phase = 0, issued = 0;
+            bool ok = true;
+            for (uint32_t i = unit; ok && i < p.items; i += units) {
+                const Item t = decode_item<EPI>(p, i);
+                const int32_t am = static_cast<int32_t>(t.tm * (128 * CG) + cta * 128);
+                for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
+                    const int32_t bn = static_cast<int32_t>(tn * BN + cta * 128);
+                    uint32_t piece = t.p0, c = 0, kb = t.p0 * p.piece;
+                    while (piece < t.p1) {
+                        const uint32_t kb1 = min((piece + 1) * p.piece, p.kblocks);
+                        const int32_t k = static_cast<int32_t>(kb * 64);
+                        const int32_t pa = static_cast<int32_t>(combo_a(c, p.combos) * p.plane_a);
+                        const int32_t pb = static_cast<int32_t>(combo_b(c, p.combos) * p.plane_b);
+                        // K blocks of a piece, then the next plane product, then the next piece.
+                        if (++kb == kb1) {
+                            kb = piece * p.piece;
+                            if (++c == p.combos) {
+                                c = 0;
+                                kb = kb1;
+                                ++piece;
+                            }
+                        }
+                        ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_limit);
+                        if (!ok) break;
+                        uint8_t* sa = stage_base + stage * kPkStageBytes;
+                        uint8_t* sb = sa + kPkStageBytes / 2;
+                        if (leader) mbar_arrive_expect_tx(&full[stage], CG * kPkStageBytes);
+                        auto load = [&](uint8_t* dst, const CUtensorMap* map, int32_t x, int32_t y) {
+                            if constexpr (CG == 2)
+                                tma_load_2d_pair(dst, map, x, y, full_leader + stage * 8);
+                            else
+                                tma_load_2d(dst, map, x, y, &full[stage]);
+                        };
+                        if constexpr (AMN) {
+                            load(sa, &map_a, pa + am, k);
+                            load(sa + 8192, &map_a, pa + am + 64, k);
+                        } else {
+                            load(sa, &map_a, pa + k, am);
+                        }
+                        if constexpr (BMN) {
+                            load(sb, &map_b, pb + bn, k);
+                            load(sb + 8192, &map_b, pb + bn + 64, k);
+                        } else {
+                            load(sb, &map_b, pb + k, bn);
+                        }
+                        ++issued;
+                        if (++stage == kPkStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                }
+            }
+            if (!ok) {
+                abort_all();
+                // Copies in flight land before the CTA's memory goes away: the
+                // last use of each stage, a bounded wait each.
+                if (leader) {
+                    for (uint32_t s = 0; s < kPkStages; ++s) {
+                        if (issued <= s) break;
+                        const uint32_t uses = (issued - s - 1) / kPkStages;  // 0-based index of its last use
+                        (void)mbar_wait_drain(&full[s], uses & 1, p.wait_limit / 8);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------ UMMA issuer
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (leader && lane == 0) {
+            const uint32_t fmt = p.in_type == kBF16 ? 1u : 0u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (AMN ? 1u << 15 : 0u) |
+                                   (BMN ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                   (static_cast<uint32_t>((128 * CG) >> 4) << 24);
+            const uint32_t s0 = smem_u32(stage_base);
+            const uint64_t a0 = AMN ? umma_desc_mn_sw128(s0) : umma_desc_sw128(s0);
+            const uint64_t b0 = BMN ? umma_desc_mn_sw128(s0 + kPkStageBytes / 2) : umma_desc_sw128(s0 + kPkStageBytes / 2);
+            constexpr uint64_t ka = AMN ? 2048 >> 4 : 2;  // 16 of K: 16 rows of 128 bytes, or 32 bytes
+            constexpr uint64_t kb = BMN ? 2048 >> 4 : 2;
+            uint32_t stage = 0, phase = 0, acc = 0;
+            bool ok = true;
+            for (uint32_t i = unit; ok && i < p.items; i += units) {
+                const Item t = decode_item<EPI>(p, i);
+                const uint32_t pieces = (t.n1 - t.n0) * (t.p1 - t.p0);
+                for (uint32_t q = 0; ok && q < pieces; ++q, ++acc) {
+                    const uint32_t piece = t.p0 + q % (t.p1 - t.p0);
+                    const uint32_t blocks = (min((piece + 1) * p.piece, p.kblocks) - piece * p.piece) * p.combos;
+                    const uint32_t buf = acc & 1u;
+                    ok = mbar_wait_sleep(&tempty[buf], ((acc >> 1) & 1u) ^ 1u, abort_flag, p.wait_limit);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + buf * BN;
+                    for (uint32_t kk = 0; kk < blocks; ++kk) {
+                        ok = mbar_wait_sleep(&full[stage], phase, abort_flag, p.wait_limit);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t ad = a0 + stage * (kPkStageBytes >> 4);
+                        const uint64_t bd = b0 + stage * (kPkStageBytes >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t more = (kk > 0 || ks > 0) ? 1u : 0u;
+                            if constexpr (CG == 2)
+                                umma_f16_pair(d, ad + ks * ka, bd + ks * kb, idesc, more);
+                            else
+                                umma_f16(d, ad + ks * ka, bd + ks * kb, idesc, more);
+                        }
+                        if constexpr (CG == 2)
+                            umma_commit_pair(&empty[stage]);
+                        else
+                            umma_commit(&empty[stage]);
+                        if (++stage == kPkStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                    }
+                    if (!ok) break;
+                    if constexpr (CG == 2)
+                        umma_commit_pair(&tfull[buf]);
+                    else
+                        umma_commit(&tfull[buf]);
+                }
+            }
+            if (!ok) abort_all();
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------ epilogue
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int e = warp - 4;
+        const uint32_t quarter = warp & 3;
+        const uint32_t half = e >> 2;
+        constexpr int kCols = BN / 2;  // columns of a tile this warp reads
+        uint8_t* box = boxes + e * 2 * kPkBox;
+        uint32_t nbox = 0;  // boxes sent: picks the buffer
+        const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(tempty), 0u) : 0u;
+        const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + half * kCols;
+        uint32_t acc = 0;
+        bool ok = true;
+
+        // The buffer of the next box, once the store that read it is done.
+        auto next_box = [&]() -> uint8_t* {
+            uint8_t* b = box + (nbox & 1u) * kPkBox;
+            ++nbox;
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+            return b;
+        };
+        // 16-byte chunk j of this thread's box row, swizzled as the TMA map expects.
+        auto put = [&](uint8_t* b, int j, uint4 v) {
+            *reinterpret_cast<uint4*>(b + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+        };
+        auto send = [&](const uint8_t* b, const CUtensorMap* map, uint32_t x, uint32_t y, bool add) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (add)
+                    tma_reduce_add_2d(map, b, static_cast<int32_t>(x), static_cast<int32_t>(y));
+                else
+                    tma_store_2d(map, b, static_cast<int32_t>(x), static_cast<int32_t>(y));
+                bulk_commit();
+            }
+            __syncwarp();
+        };
+        // Element stores of a box of `esize`-byte values to rows that TMA cannot write.
+        auto copy_out = [&](const uint8_t* b, void* dst, uint64_t ld, int esize, uint32_t row0, uint32_t col0) {
+            __syncwarp();
+            const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
+            const uint32_t cols = 128u / esize;
+            for (uint32_t r = 0; r < rows; ++r) {
+                for (uint32_t c = lane; c < cols; c += 32) {
+                    if (col0 + c >= p.n) continue;
+                    const uint32_t byte = c * esize;
+                    const uint8_t* src = b + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
+                    const uint64_t at = (row0 + r) * ld + col0 + c;
+                    if (esize == 2)
+                        static_cast<uint16_t*>(dst)[at] = *reinterpret_cast<const uint16_t*>(src);
+                    else
+                        static_cast<uint32_t*>(dst)[at] = *reinterpret_cast<const uint32_t*>(src);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) bulk_commit();  // an empty group: the buffers keep taking turns
+        };
+        // The tensor cores add into TMEM by truncation, which over a long K
+        // pulls every sum towards zero by parts in 10^5. So K is summed there
+        // in pieces, and the pieces are added in registers, rounded to nearest.
+        float sums[LONG ? kCols : 1];
+        // Columns [c, c + 32) of the last piece, the earlier ones added.
+        auto load32 = [&](uint32_t buf, int c, float* v) {
+            int32_t* r = reinterpret_cast<int32_t*>(v);
+            tmem_ld_32cols(lane_base + buf * BN + c, r);
+            tmem_ld_wait_n<32>(r);
+            if constexpr (LONG) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += sums[c + j];
+            }
+        };
+        auto release = [&](uint32_t buf) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    mbar_arrive_remote(tempty_leader + buf * 8);
+                else
+                    mbar_arrive(&tempty[buf]);
+            }
+        };
+
+        // The buffer with the last K piece of a tile, after the earlier pieces
+        // went into `sums`.
+        auto tile_ready = [&](uint32_t pieces, uint32_t& buf) -> bool {
+            if constexpr (LONG) {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sums[j] = 0.0f;
+                for (uint32_t q = 1; q < pieces; ++q) {
+                    buf = acc & 1u;
+                    if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, p.wait_limit)) return false;
+                    ++acc;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        float v[32];
+                        load32(buf, c, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sums[c + j] = v[j];
+                    }
+                    release(buf);
+                }
+            }
+            buf = acc & 1u;
+            if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, p.wait_limit)) return false;
+            ++acc;
+            tc_fence_after();
+            return true;
+        };
+        constexpr int kUnroll = LONG ? kCols / 32 : 1;  // `sums` needs constant indices
+        constexpr int kUnroll2 = LONG ? kCols / 64 : 1;
+
+        for (uint32_t i = unit; ok && i < p.items; i += units) {
+            const Item t = decode_item<EPI>(p, i);
+            const uint32_t row0 = t.tm * (128 * CG) + cta * 128 + quarter * 32;
+            const uint32_t row = row0 + lane;
+            const bool live = row < p.m;
+
+            if constexpr (EPI == kEpiStore) {
+                const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
+                uint32_t buf;
+                ok = tile_ready(t.p1 - t.p0, buf);
+                if (!ok) break;
+                const uint32_t col_base = t.n0 * BN + half * kCols;
+                const uint32_t out_row0 = row0 + t.split * p.split_rows;
+                const int osize = p.out_type == kF32 ? 4 : 2;
+                uint4 keep[4];  // first half of a 16-bit box
+#pragma unroll kUnroll
+                for (int c = 0; c < kCols; c += 32) {
+                    float v[32];
+                    load32(buf, c, v);
+                    if (c + 32 == kCols) release(buf);
+                    const uint32_t col = col_base + c;
+                    if (alpha != 1.0f) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= alpha;
+                    }
+                    if (p.bias) {
+                        if (col + 32 <= p.n) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += load_elem(p.bias, col + j, p.aux_type);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (col + j < p.n) v[j] += load_elem(p.bias, col + j, p.aux_type);
+                        }
+                    }
+                    if (p.pre) {
+                        // The value before the activation, rounded to the inputs' type.
+                        if (p.aux_type == kF32) {
+                            uint8_t* b = next_box();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                put(b, j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                     __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+                            if (p.pre_tma)
+                                send(b, &map_pre, col, row0, false);
+                            else
+                                copy_out(b, p.pre, p.ldp, 4, row0, col);
+                        } else {
+                            // Half a box (32 columns = 64 bytes a row): the map's boxes are 32 columns wide.
+                            uint8_t* b = next_box();
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                *reinterpret_cast<uint4*>(b + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                                    make_uint4(pack2(v[8 * j], v[8 * j + 1], p.aux_type),
+                                               pack2(v[8 * j + 2], v[8 * j + 3], p.aux_type),
+                                               pack2(v[8 * j + 4], v[8 * j + 5], p.aux_type),
+                                               pack2(v[8 * j + 6], v[8 * j + 7], p.aux_type));
+                            if (p.pre_tma) {
+                                send(b, &map_pre, col, row0, false);
+                            } else {
+                                __syncwarp();
+                                const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
+                                for (uint32_t r = 0; r < rows; ++r) {
+                                    if (col + lane >= p.n) continue;
+                                    const uint32_t byte = lane * 2;
+                                    static_cast<uint16_t*>(p.pre)[(row0 + r) * p.ldp + col + lane] =
+                                        *reinterpret_cast<const uint16_t*>(
+                                            b + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
+                                }
+                                __syncwarp();
+                                if (lane == 0) bulk_commit();
+                            }
+                        }
+                    }
+                    switch (p.activation) {
+                        case kActRelu: act_all<kActRelu>(v); break;
+                        case kActGelu: act_all<kActGelu>(v); break;
+                        case kActGeluTanh: act_all<kActGeluTanh>(v); break;
+                        case kActSilu: act_all<kActSilu>(v); break;
+                        default: break;
+                    }
+                    if (p.residual && live) {
+                        const uint64_t at = row * p.ldr + col;
+                        if (p.residual_vec && col + 32 <= p.n) {
+                            if (p.aux_type == kF32) {
+                                const float4* r4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float4 q = r4[j];
+                                    v[4 * j] += q.x;
+                                    v[4 * j + 1] += q.y;
+                                    v[4 * j + 2] += q.z;
+                                    v[4 * j + 3] += q.w;
+                                }
+                            } else {
+                                const uint4* r4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint4 q = r4[j];
+                                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                                    for (int h = 0; h < 4; ++h) {
+                                        const float2 f = unpack2(w[h], p.aux_type);
+                                        v[8 * j + 2 * h] += f.x;
+                                        v[8 * j + 2 * h + 1] += f.y;
+                                    }
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (col + j < p.n) v[j] += load_elem(p.residual, at + j, p.aux_type);
+                        }
+                    }
+                    if (osize == 4) {
+                        uint8_t* b = next_box();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            put(b, j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                                 __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+                        if (p.out_tma)
+                            send(b, &map_out, col, out_row0, p.accumulate != 0);
+                        else
+                            copy_out(b, p.out, p.ldo, 4, row0, col);
+                    } else {
+                        uint4 now[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            now[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1], p.out_type),
+                                                pack2(v[8 * j + 2], v[8 * j + 3], p.out_type),
+                                                pack2(v[8 * j + 4], v[8 * j + 5], p.out_type),
+                                                pack2(v[8 * j + 6], v[8 * j + 7], p.out_type));
+                        if ((c & 32) == 0) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) keep[j] = now[j];
+                        } else {
+                            uint8_t* b = next_box();
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                put(b, j, keep[j]);
+                                put(b, j + 4, now[j]);
+                            }
+                            if (p.out_tma)
+                                send(b, &map_out, col - 32, out_row0, false);
+                            else
+                                copy_out(b, p.out, p.ldo, 2, row0, col - 32);
+                        }
+                    }
+                }
+            } else if constexpr (EPI == kEpiSoftmax) {
+                // Running maximum (of the scaled logits, base 2) and sum of
+                // 2^(logit - maximum) of this row over its half of the columns,
+                // the label's column left out.
+                float top = -INFINITY, sum = 0.0f;
+                const int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
+                for (uint32_t tn = t.n0; tn < t.n1; ++tn) {
+                    uint32_t buf;
+                    ok = tile_ready(t.p1 - t.p0, buf);
+                    if (!ok) break;
+                    const uint32_t col_base = tn * BN + half * kCols;
+#pragma unroll kUnroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        float v[32];
+                        load32(buf, c, v);
+                        if (c + 32 == kCols) release(buf);
+                        const uint32_t col = col_base + c;
+                        const int32_t at = label - static_cast<int32_t>(col);
+                        if (at >= 0 && at < 32) {
+                            float z = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                z = j == at ? v[j] : z;
+                                v[j] = j == at ? -INFINITY : v[j];  // its term is added by the join
+                            }
+                            p.label_dot[row] = z;
+                        }
+                        if (col + 32 > p.n) {  // past the last column: no weight
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (col + j >= p.n) v[j] = -INFINITY;
+                        }
+                        float big = v[0];
+#pragma unroll
+                        for (int j = 1; j < 32; ++j) big = fmaxf(big, v[j]);
+                        const float now = fmaxf(top, big * p.scale2);
+                        // A row whose logits so far are all -inf has no sum yet.
+                        const float base = now == -INFINITY ? 0.0f : now;
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(v[j], p.scale2, -base));
+                        sum = sum * exp2_approx(top - base) + ((part[0] + part[1]) + (part[2] + part[3]));
+                        top = now;
+                    }
+                }
+                if (ok && live) p.part[uint64_t(2 * t.segment + half) * p.m + row] = make_float2(top, sum);
+            } else {
+                const float lse2 = live ? p.lse2[row] : 0.0f;
+                float cmax_inv = 1.0f;
+                if (p.alpha_dev) cmax_inv = *p.alpha_dev > 0.0f ? 1.0f / *p.alpha_dev : 0.0f;
+                const float coef = live ? p.coef[row] * cmax_inv * p.grad_scale : 0.0f;
+                // Column of the row's class here; negative where it has none or an earlier piece holds it.
+                int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
+                if (label >= 0) label -= static_cast<int32_t>(p.class0);
+                uint32_t buf;
+                ok = tile_ready(t.p1 - t.p0, buf);
+                if (!ok) break;
+                const uint32_t col_base = t.n0 * BN + half * kCols;
+#pragma unroll kUnroll2
+                for (int c = 0; c < kCols; c += 64) {
+                    uint4 lo[8], mid[8], low[8];
+                    const uint32_t col0 = col_base + c;
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        float v[32];
+                        load32(buf, c + 32 * hh, v);
+                        if (c + 32 * hh + 32 == kCols) release(buf);
+                        const uint32_t col = col0 + 32 * hh;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = coef * exp2_approx(fmaf(v[j], p.scale2, -lse2));
+                        const int32_t at = label - static_cast<int32_t>(col);
+                        if (at >= 0 && at < 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j == at) v[j] -= coef;
+                        }
+                        if (p.grad_planes == 3 && col + 32 > p.n) {  // pad columns of a plane hold zeros
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (col + j >= p.n) v[j] = 0.0f;
+                        }
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], p.in_type);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            lo[4 * hh + j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                        if (p.grad_planes == 3) {
+                            uint32_t wm[16], wl[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                float2 f = unpack2(w[j], kBF16);
+                                const float r0 = v[2 * j] - f.x, r1 = v[2 * j + 1] - f.y;
+                                wm[j] = pack2(r0, r1, kBF16);
+                                f = unpack2(wm[j], kBF16);
+                                wl[j] = pack2(r0 - f.x, r1 - f.y, kBF16);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                mid[4 * hh + j] = make_uint4(wm[4 * j], wm[4 * j + 1], wm[4 * j + 2], wm[4 * j + 3]);
+                                low[4 * hh + j] = make_uint4(wl[4 * j], wl[4 * j + 1], wl[4 * j + 2], wl[4 * j + 3]);
+                            }
+                        }
+                    }
+                    if (p.grad_planes == 1) {
+                        uint8_t* b = next_box();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) put(b, j, lo[j]);
+                        send(b, &map_out, col0, row0, false);
+                    } else if (col0 < p.grad_pitch) {
+                        uint8_t* b = next_box();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) put(b, j, lo[j]);
+                        send(b, &map_out, col0, row0, false);
+                        b = next_box();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) put(b, j, mid[j]);
+                        send(b, &map_out, p.grad_pitch + col0, row0, false);
+                        b = next_box();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) put(b, j, low[j]);
+                        send(b, &map_out, 2 * p.grad_pitch + col0, row0, false);
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0) abort_all();
+        if (lane == 0) bulk_wait_all();
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    }
+
+    tc_fence_before();
+    if constexpr (CG == 2)
+        cluster_sync_all();
+    else
+        __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        if constexpr (CG == 2)
+            tmem_dealloc_pair(tmem_base, kTmemCols);
+        else
+            tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+}  // namespace knng_b200
