@@ -97,6 +97,10 @@ struct JoinParams {
     const void* labels;     // rows without a label become zeros
     int labels_i64;
     uint32_t classes;
+    const float* label_rest;  // with labels: row r also gets label_rest[r] * (row `label` of w), 16-bit rows
+    const void* w;
+    uint64_t ldw;
+    int w_type;
 };
 
 // The pieces of a split product, summed in order, and the linear epilogue.
@@ -109,10 +113,17 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const JoinParams p)
         const uint64_t r = i / groups;
         const uint32_t c = static_cast<uint32_t>(i - r * groups) * 4;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (!p.labels || load_label(p.labels, p.labels_i64, r, p.classes) >= 0) {
+        const int32_t label = p.labels ? load_label(p.labels, p.labels_i64, r, p.classes) : 0;
+        if (label >= 0) {
             for (uint32_t s = 0; s < p.splits; ++s) {
                 const float4 q = *reinterpret_cast<const float4*>(p.part + (s * p.split_rows + r) * p.pitch + c);
                 v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            }
+            if (p.label_rest) {
+                const float rest = p.label_rest[r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < p.n) v[j] = fmaf(rest, load_elem(p.w, label * p.ldw + c + j, p.w_type), v[j]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] *= alpha;
@@ -206,12 +217,10 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
 struct SlopeParams {
     const void* dy;
     uint64_t lddy;
-    const void* pre;      // may be NULL: dz = dy
+    const void* pre;      // not read without an activation
     uint64_t ldp;
     uint64_t m;
     uint32_t n;
-    int type;
-    int activation;
     uint16_t* out;        // dz as 16-bit operands (may be NULL: column sums only)
     uint32_t pitch;       // columns of a plane of out
     uint32_t planes;
@@ -245,7 +254,9 @@ __device__ __forceinline__ void load8(const void* p, uint64_t at, int type, uint
 
 // dz = dy act'(pre), rounded to the operands' type, and its column sums (of
 // the unrounded values). A block takes 256 columns (8 per lane) and a range of
-// rows; its 8 warps take every eighth row and add up their sums in order.
+// rows; its 8 warps take every eighth row, two at a time so that four 16-byte
+// loads a thread are in flight, and add up their sums in order.
+template <int ACT, int TYPE>
 __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
 {
     __shared__ float total[8][256];
@@ -253,43 +264,39 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
     const uint32_t c0 = blockIdx.x * 256 + lane * 8;
     const uint64_t r0 = p.m * blockIdx.y / gridDim.y, r1 = p.m * (blockIdx.y + 1) / gridDim.y;
     const uint32_t left = c0 < p.n ? p.n - c0 : 0;
+    const bool whole = p.vec && left >= 8;
     float acc[8] = {};
-    for (uint64_t r = r0 + warp; r < r1; r += 8) {
-        float v[8] = {};
-        if (left) {
-            load8(p.dy, r * p.lddy + c0, p.type, left, p.vec, v);
-            if (p.pre) {
-                float z[8];
-                load8(p.pre, r * p.ldp + c0, p.type, left, p.vec, z);
-                const uint32_t have = left < 8 ? left : 8;
+    for (uint64_t r = r0 + warp; r < r1; r += 16) {
+        float v[2][8] = {}, z[2][8] = {};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j >= static_cast<int>(have)) break;
-                    switch (p.activation) {
-                        case kActRelu: v[j] *= slope_f<kActRelu>(z[j]); break;
-                        case kActGelu: v[j] *= slope_f<kActGelu>(z[j]); break;
-                        case kActGeluTanh: v[j] *= slope_f<kActGeluTanh>(z[j]); break;
-                        case kActSilu: v[j] *= slope_f<kActSilu>(z[j]); break;
-                        default: break;
-                    }
-                }
+        for (int h = 0; h < 2; ++h) {
+            if (left && r + 8 * h < r1) {
+                load8(p.dy, (r + 8 * h) * p.lddy + c0, TYPE, left, whole, v[h]);
+                if constexpr (ACT != kActNone) load8(p.pre, (r + 8 * h) * p.ldp + c0, TYPE, left, whole, z[h]);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += v[j];
         }
-        if (p.out && c0 < p.pitch) {
-            uint16_t* dst = p.out + r * (uint64_t(p.pitch) * p.planes) + c0;
-            for (uint32_t plane = 0; plane < p.planes; ++plane) {
-                uint32_t w[4];
-                const int type = p.type == kF16 ? kF16 : kBF16;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    w[j] = pack2(v[2 * j], v[2 * j + 1], type);
-                    const float2 f = unpack2(w[j], type);
-                    v[2 * j] -= f.x;
-                    v[2 * j + 1] -= f.y;
+        for (int h = 0; h < 2; ++h) {
+            if (r + 8 * h >= r1) break;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (ACT != kActNone) v[h][j] *= slope_f<ACT>(z[h][j]);
+                acc[j] += v[h][j];
+            }
+            if (p.out && c0 < p.pitch) {
+                uint16_t* dst = p.out + (r + 8 * h) * (uint64_t(p.pitch) * p.planes) + c0;
+                constexpr int kOut = TYPE == kF16 ? kF16 : kBF16;
+                for (uint32_t plane = 0; plane < p.planes; ++plane) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[j] = pack2(v[h][2 * j], v[h][2 * j + 1], kOut);
+                        const float2 f = unpack2(w[j], kOut);
+                        v[h][2 * j] -= f.x;
+                        v[h][2 * j + 1] -= f.y;
+                    }
+                    *reinterpret_cast<uint4*>(dst + plane * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                *reinterpret_cast<uint4*>(dst + plane * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }

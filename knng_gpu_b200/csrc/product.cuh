@@ -13,18 +13,19 @@
 // leading one, summed smallest first into the same accumulator; the three that
 // are left out are below 2^-26 of it.
 //
-// Tile and roles. CG = 2: a CTA pair computes 256 x 256 with
-// tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and 128 of B per
-// 64-wide K block, half of what two single-CTA tiles would read from L2.
-// CG = 1: 128 x 128 by one CTA, for products with too few tiles to fill the
+// Tile and roles. CG = 2: a CTA pair computes up to 256 x 256 with
+// tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and half the tile's
+// rows of B per 64-wide K block, half of what two single-CTA tiles would read
+// from L2. CG = 1: up to 128 x 128 by one CTA, for products with too few tiles to fill the
 // GPU with pairs. Per CTA:
 //   warp 0      TMA producer, kStages-deep ring of 32 KiB stages
 //   warp 1      TMEM allocation; UMMA issue (leader CTA, one lane)
 //   warps 2-3   idle
-//   warps 4-11  epilogue: thread = one accumulator row, the two halves of the
-//               warps take the two halves of the columns. Two accumulator
-//               buffers in TMEM: the epilogue of a tile runs under the MMAs of
-//               the next one.
+//   warps 4-11  epilogue: thread = one accumulator row; the first four warps
+//               take the even 32-column chunks of a tile, the others the odd
+//               ones, each loading a chunk from TMEM while it works on the
+//               one before. Two accumulator buffers in TMEM: the epilogue of
+//               a tile runs under the MMAs of the next one.
 // Outputs leave through 4 KiB shared-memory boxes per warp and TMA stores
 // (reduce-adds where a call accumulates), or by coalesced element stores where
 // the output rows are not 16-byte aligned.
@@ -43,7 +44,7 @@ constexpr int kPkThreads = 384;    // 4 + 8 warps
 constexpr int kPkEpiWarps = 8;
 constexpr int kPkStages = 5;
 constexpr int kPkStageBytes = 32768;  // 128 x 64 of A and of B, 2 bytes each
-constexpr int kPkBox = 4096;          // staging box: 32 rows x 128 bytes
+constexpr int kPkBox = 4096;          // staging box: 32 rows x 32 columns of 4 (or 2) bytes
 constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkEpiWarps * 2 * kPkBox + 512 + 1024;
 
 enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
@@ -52,6 +53,7 @@ enum Epilogue : int { kEpiStore = 0, kEpiSoftmax = 1, kEpiGrad = 2 };
 
 struct ProductParams {
     uint32_t m, n;                 // rows and columns of D
+    uint32_t tile_n;               // columns of a tile: a multiple of 32, at most 128 * CG
     uint32_t tiles_m, tiles_n;
     uint32_t splits;               // store: pieces of the K loop, each to its own rows of the output map
     uint32_t segments;             // softmax: pieces of the columns per row tile
@@ -75,7 +77,7 @@ struct ProductParams {
     const void* residual;
     uint64_t ldr;
     int aux_type;
-    int residual_vec;              // residual rows allow 16-byte loads
+    int bias_vec, residual_vec;    // they allow 16-byte loads
     int activation;
     float alpha;                   // D is scaled by alpha * *alpha_dev
     const float* alpha_dev;
@@ -91,6 +93,7 @@ struct ProductParams {
     const float* coef;             // gradient: dloss * scale / cmax, 0 for a row without label
     float grad_scale;              // gradient: power of two on the stored values
     uint32_t grad_planes, grad_pitch;
+    float* label_rest;             // gradient: what rounding took from the label's entry (one plane)
 };
 
 // ---------------------------------------------------------------- PTX of this kernel
@@ -191,15 +194,42 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, int type)
     return __half22float2(h);
 }
 
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // sigmoid(v) = 1 / (1 + e^-v); e^-v overflows to +inf for very negative v,
 // where the quotient is 0 as it should be.
-__device__ __forceinline__ float sigmoid_f(float v) { return 1.0f / (1.0f + exp2_approx(-1.44269504f * v)); }
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.0f + exp2_approx(-1.44269504f * v)); }
+
+// The normal distribution function Phi(z) and *bell = e^(-z^2 / 2), by
+// Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2) with
+// t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7 for x = |z| / sqrt 2 >= 0.
+// No branch, and the gradient needs the same exponential.
+__device__ __forceinline__ float normal_cdf(float z, float* bell)
+{
+    const float e = exp2_approx(-0.72134752f * z * z);
+    const float t = rcp_approx(fmaf(fabsf(z), 0.23164189f, 1.0f));
+    float q = fmaf(t, 0.530702715f, -0.726576014f);  // half the coefficients: Phi(-|z|) = erfc(x) / 2
+    q = fmaf(t, q, 0.710706871f);
+    q = fmaf(t, q, -0.142248368f);
+    q = fmaf(t, q, 0.127414796f);
+    q = q * t * e;
+    *bell = e;
+    return z < 0.0f ? q : 1.0f - q;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float z)
 {
     if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    if constexpr (ACT == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    if constexpr (ACT == kActGelu) {
+        float bell;
+        return z * normal_cdf(z, &bell);
+    }
     // 0.5 (1 + tanh u) = sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3).
     if constexpr (ACT == kActGeluTanh) return z * sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
     if constexpr (ACT == kActSilu) return z * sigmoid_f(z);
@@ -210,8 +240,11 @@ template <int ACT>
 __device__ __forceinline__ float slope_f(float z)
 {
     if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
-    if constexpr (ACT == kActGelu)
-        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * exp2_approx(-0.72134752f * z * z);
+    if constexpr (ACT == kActGelu) {
+        float bell;
+        const float phi = normal_cdf(z, &bell);
+        return fmaf(0.39894228f * z, bell, phi);
+    }
     if constexpr (ACT == kActGeluTanh) {
         const float s = sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
         return s + z * s * (1.0f - s) * 1.59576912f * (1.0f + 0.134145f * z * z);
@@ -232,6 +265,44 @@ __device__ __forceinline__ float act_dyn(float z, int act)
         case kActGeluTanh: return act_f<kActGeluTanh>(z);
         case kActSilu: return act_f<kActSilu>(z);
         default: return z;
+    }
+}
+
+// 32 values as 16 words of two.
+__device__ __forceinline__ void pack32(const float* v, uint32_t* w, int type)
+{
+    if (type == kBF16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], kBF16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], kF16);
+    }
+}
+
+// Adds 32 consecutive 16-bit values.
+__device__ __forceinline__ void add_words(float* v, const uint4* src, int type)
+{
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint4 q = src[j];
+        w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
+    }
+    if (type == kBF16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float2 f = unpack2(w[j], kBF16);
+            v[2 * j] += f.x;
+            v[2 * j + 1] += f.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float2 f = unpack2(w[j], kF16);
+            v[2 * j] += f.x;
+            v[2 * j + 1] += f.y;
+        }
     }
 }
 
@@ -307,8 +378,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                    const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
                    const ProductParams p)
 {
-    constexpr int BN = 128 * CG;           // columns of a tile
-    constexpr uint32_t kTmemCols = 2 * BN;
+    constexpr uint32_t kBufCols = 128 * CG;  // TMEM columns of an accumulator buffer
+    constexpr uint32_t kTmemCols = 2 * kBufCols;
+    const uint32_t bn_tile = p.tile_n;
+    const uint32_t bn_cta = bn_tile / CG;    // rows of B that this CTA stages
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stage_base = smem;
@@ -370,13 +443,15 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (lane == 0) {
             const uint32_t full_leader = CG == 2 ? mapa_shared(smem_u32(full), 0u) : 0u;
+            const uint32_t b_bytes = BMN ? (bn_cta > 64 ? 16384u : 8192u) : bn_cta * 128u;
+            const uint32_t tx = CG * (kPkStageBytes / 2 + b_bytes);
             uint32_t stage = 0, phase = 0, issued = 0;
             bool ok = true;
             for (uint32_t i = unit; ok && i < p.items; i += units) {
                 const Item t = decode_item<EPI>(p, i);
                 const int32_t am = static_cast<int32_t>(t.tm * (128 * CG) + cta * 128);
                 for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
-                    const int32_t bn = static_cast<int32_t>(tn * BN + cta * 128);
+                    const int32_t bn = static_cast<int32_t>(tn * bn_tile + cta * bn_cta);
                     uint32_t piece = t.p0, c = 0, kb = t.p0 * p.piece;
                     while (piece < t.p1) {
                         const uint32_t kb1 = min((piece + 1) * p.piece, p.kblocks);
@@ -396,7 +471,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         if (!ok) break;
                         uint8_t* sa = stage_base + stage * kPkStageBytes;
                         uint8_t* sb = sa + kPkStageBytes / 2;
-                        if (leader) mbar_arrive_expect_tx(&full[stage], CG * kPkStageBytes);
+                        if (leader) mbar_arrive_expect_tx(&full[stage], tx);
                         auto load = [&](uint8_t* dst, const CUtensorMap* map, int32_t x, int32_t y) {
                             if constexpr (CG == 2)
                                 tma_load_2d_pair(dst, map, x, y, full_leader + stage * 8);
@@ -411,7 +486,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         }
                         if constexpr (BMN) {
                             load(sb, &map_b, pb + bn, k);
-                            load(sb + 8192, &map_b, pb + bn + 64, k);
+                            if (bn_cta > 64) load(sb + 8192, &map_b, pb + bn + 64, k);
                         } else {
                             load(sb, &map_b, pb + k, bn);
                         }
@@ -443,7 +518,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (leader && lane == 0) {
             const uint32_t fmt = p.in_type == kBF16 ? 1u : 0u;
             const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (AMN ? 1u << 15 : 0u) |
-                                   (BMN ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                   (BMN ? 1u << 16 : 0u) | ((bn_tile >> 3) << 17) |
                                    (static_cast<uint32_t>((128 * CG) >> 4) << 24);
             const uint32_t s0 = smem_u32(stage_base);
             const uint64_t a0 = AMN ? umma_desc_mn_sw128(s0) : umma_desc_sw128(s0);
@@ -462,7 +537,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     ok = mbar_wait_sleep(&tempty[buf], ((acc >> 1) & 1u) ^ 1u, abort_flag, p.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d = tmem_base + buf * BN;
+                    const uint32_t d = tmem_base + buf * kBufCols;
                     for (uint32_t kk = 0; kk < blocks; ++kk) {
                         ok = mbar_wait_sleep(&full[stage], phase, abort_flag, p.wait_limit);
                         if (!ok) break;
@@ -502,11 +577,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const int e = warp - 4;
         const uint32_t quarter = warp & 3;
         const uint32_t half = e >> 2;
-        constexpr int kCols = BN / 2;  // columns of a tile this warp reads
+        constexpr int kMaxChunks = 2 * CG;  // 32-column chunks per warp: 0, 2, .. or 1, 3, ..
+        const int chunks = static_cast<int>((bn_tile / 32 + 1 - half) / 2);
         uint8_t* box = boxes + e * 2 * kPkBox;
         uint32_t nbox = 0;  // boxes sent: picks the buffer
         const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(tempty), 0u) : 0u;
-        const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + half * kCols;
+        const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + half * 32;
         uint32_t acc = 0;
         bool ok = true;
 
@@ -518,9 +594,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             __syncwarp();
             return b;
         };
-        // 16-byte chunk j of this thread's box row, swizzled as the TMA map expects.
-        auto put = [&](uint8_t* b, int j, uint4 v) {
-            *reinterpret_cast<uint4*>(b + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+        // This thread's row of a box, swizzled as the TMA maps expect: 32 fp32
+        // values in 128-byte rows, or 32 16-bit values (16 words) in 64-byte rows.
+        auto put_f32 = [&](uint8_t* b, const float* v) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4*>(b + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                    make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                               __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+        };
+        auto put_words = [&](uint8_t* b, const uint32_t* w) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(b + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         };
         auto send = [&](const uint8_t* b, const CUtensorMap* map, uint32_t x, uint32_t y, bool add) {
             fence_proxy_async_smem();
@@ -534,40 +621,28 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             }
             __syncwarp();
         };
-        // Element stores of a box of `esize`-byte values to rows that TMA cannot write.
+        // Element stores of a box to rows that TMA cannot write.
         auto copy_out = [&](const uint8_t* b, void* dst, uint64_t ld, int esize, uint32_t row0, uint32_t col0) {
             __syncwarp();
             const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
-            const uint32_t cols = 128u / esize;
-            for (uint32_t r = 0; r < rows; ++r) {
-                for (uint32_t c = lane; c < cols; c += 32) {
-                    if (col0 + c >= p.n) continue;
-                    const uint32_t byte = c * esize;
-                    const uint8_t* src = b + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
-                    const uint64_t at = (row0 + r) * ld + col0 + c;
+            if (col0 + lane < p.n) {
+                for (uint32_t r = 0; r < rows; ++r) {
+                    const uint64_t at = (row0 + r) * ld + col0 + lane;
                     if (esize == 2)
-                        static_cast<uint16_t*>(dst)[at] = *reinterpret_cast<const uint16_t*>(src);
+                        static_cast<uint16_t*>(dst)[at] = *reinterpret_cast<const uint16_t*>(
+                            b + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
                     else
-                        static_cast<uint32_t*>(dst)[at] = *reinterpret_cast<const uint32_t*>(src);
+                        static_cast<uint32_t*>(dst)[at] = *reinterpret_cast<const uint32_t*>(
+                            b + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
                 }
             }
             __syncwarp();
             if (lane == 0) bulk_commit();  // an empty group: the buffers keep taking turns
         };
-        // The tensor cores add into TMEM by truncation, which over a long K
-        // pulls every sum towards zero by parts in 10^5. So K is summed there
-        // in pieces, and the pieces are added in registers, rounded to nearest.
-        float sums[LONG ? kCols : 1];
-        // Columns [c, c + 32) of the last piece, the earlier ones added.
-        auto load32 = [&](uint32_t buf, int c, float* v) {
-            int32_t* r = reinterpret_cast<int32_t*>(v);
-            tmem_ld_32cols(lane_base + buf * BN + c, r);
-            tmem_ld_wait_n<32>(r);
-            if constexpr (LONG) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += sums[c + j];
-            }
+        auto issue = [&](uint32_t buf, int i, float* v) {
+            tmem_ld_32cols(lane_base + buf * kBufCols + i * 64, reinterpret_cast<int32_t*>(v));
         };
+        auto arrived = [&](float* v) { tmem_ld_wait_n<32>(reinterpret_cast<int32_t*>(v)); };
         auto release = [&](uint32_t buf) {
             tc_fence_before();
             __syncwarp();
@@ -578,66 +653,105 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     mbar_arrive(&tempty[buf]);
             }
         };
-
-        // The buffer with the last K piece of a tile, after the earlier pieces
-        // went into `sums`.
-        auto tile_ready = [&](uint32_t pieces, uint32_t& buf) -> bool {
-            if constexpr (LONG) {
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) sums[j] = 0.0f;
-                for (uint32_t q = 1; q < pieces; ++q) {
-                    buf = acc & 1u;
-                    if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, p.wait_limit)) return false;
-                    ++acc;
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < kCols; c += 32) {
-                        float v[32];
-                        load32(buf, c, v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sums[c + j] = v[j];
-                    }
-                    release(buf);
-                }
-            }
+        auto wait_acc = [&](uint32_t& buf) -> bool {
             buf = acc & 1u;
             if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, p.wait_limit)) return false;
             ++acc;
             tc_fence_after();
             return true;
         };
-        constexpr int kUnroll = LONG ? kCols / 32 : 1;  // `sums` needs constant indices
-        constexpr int kUnroll2 = LONG ? kCols / 64 : 1;
+        // Calls f(v, chunk) for this warp's chunks of the next tile, whose sums
+        // are in v. The tensor cores add into TMEM by truncation, which over a
+        // long K pulls every sum towards zero by parts in 10^5: K is summed
+        // there in pieces, and the pieces are added in registers, rounded to
+        // nearest.
+        auto for_tile = [&](uint32_t pieces, auto&& f) -> bool {
+            uint32_t buf;
+            if constexpr (!LONG) {
+                if (!wait_acc(buf)) return false;
+                float va[32], vb[32];
+                issue(buf, 0, va);
+#pragma unroll 1
+                for (int i = 0; i < chunks; i += 2) {
+                    arrived(va);
+                    if (i + 1 < chunks)
+                        issue(buf, i + 1, vb);
+                    else
+                        release(buf);
+                    f(va, i);
+                    if (i + 1 < chunks) {
+                        arrived(vb);
+                        if (i + 2 < chunks)
+                            issue(buf, i + 2, va);
+                        else
+                            release(buf);
+                        f(vb, i + 1);
+                    }
+                }
+            } else {
+                float sums[32 * kMaxChunks];
+#pragma unroll
+                for (int j = 0; j < 32 * kMaxChunks; ++j) sums[j] = 0.0f;
+                for (uint32_t q = 0; q < pieces; ++q) {
+                    if (!wait_acc(buf)) return false;
+                    float va[32], vb[32];
+                    issue(buf, 0, va);
+#pragma unroll
+                    for (int i = 0; i < kMaxChunks; i += 2) {
+                        arrived(va);
+                        if (i + 1 < chunks) issue(buf, i + 1, vb);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sums[32 * i + j] += va[j];
+                        if (i + 1 < chunks) {
+                            arrived(vb);
+                            if (i + 2 < chunks) issue(buf, i + 2, va);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sums[32 * i + 32 + j] += vb[j];
+                        }
+                        if (i + 2 >= chunks) break;
+                    }
+                    release(buf);
+                }
+#pragma unroll
+                for (int i = 0; i < kMaxChunks; ++i)
+                    if (i < chunks) f(sums + 32 * i, i);
+            }
+            return true;
+        };
 
-        for (uint32_t i = unit; ok && i < p.items; i += units) {
-            const Item t = decode_item<EPI>(p, i);
+        for (uint32_t it = unit; ok && it < p.items; it += units) {
+            const Item t = decode_item<EPI>(p, it);
             const uint32_t row0 = t.tm * (128 * CG) + cta * 128 + quarter * 32;
             const uint32_t row = row0 + lane;
             const bool live = row < p.m;
 
             if constexpr (EPI == kEpiStore) {
                 const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
-                uint32_t buf;
-                ok = tile_ready(t.p1 - t.p0, buf);
-                if (!ok) break;
-                const uint32_t col_base = t.n0 * BN + half * kCols;
+                const uint32_t col_base = t.n0 * bn_tile + half * 32;
                 const uint32_t out_row0 = row0 + t.split * p.split_rows;
-                const int osize = p.out_type == kF32 ? 4 : 2;
-                uint4 keep[4];  // first half of a 16-bit box
-#pragma unroll kUnroll
-                for (int c = 0; c < kCols; c += 32) {
-                    float v[32];
-                    load32(buf, c, v);
-                    if (c + 32 == kCols) release(buf);
-                    const uint32_t col = col_base + c;
+                ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
+                    const uint32_t col = col_base + i * 64;
+                    if (row0 >= p.m || col >= p.n) return;  // nobody reads what lies there
                     if (alpha != 1.0f) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] *= alpha;
                     }
                     if (p.bias) {
-                        if (col + 32 <= p.n) {
+                        if (p.bias_vec && col + 32 <= p.n) {
+                            if (p.aux_type == kF32) {
+                                const float4* q4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] += load_elem(p.bias, col + j, p.aux_type);
+                                for (int j = 0; j < 8; ++j) {
+                                    const float4 q = q4[j];
+                                    v[4 * j] += q.x;
+                                    v[4 * j + 1] += q.y;
+                                    v[4 * j + 2] += q.z;
+                                    v[4 * j + 3] += q.w;
+                                }
+                            } else {
+                                add_words(v, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + col),
+                                          p.aux_type);
+                            }
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
@@ -646,42 +760,18 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                     if (p.pre) {
                         // The value before the activation, rounded to the inputs' type.
+                        uint8_t* b = next_box();
                         if (p.aux_type == kF32) {
-                            uint8_t* b = next_box();
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                put(b, j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                     __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
-                            if (p.pre_tma)
-                                send(b, &map_pre, col, row0, false);
-                            else
-                                copy_out(b, p.pre, p.ldp, 4, row0, col);
+                            put_f32(b, v);
                         } else {
-                            // Half a box (32 columns = 64 bytes a row): the map's boxes are 32 columns wide.
-                            uint8_t* b = next_box();
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                *reinterpret_cast<uint4*>(b + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                                    make_uint4(pack2(v[8 * j], v[8 * j + 1], p.aux_type),
-                                               pack2(v[8 * j + 2], v[8 * j + 3], p.aux_type),
-                                               pack2(v[8 * j + 4], v[8 * j + 5], p.aux_type),
-                                               pack2(v[8 * j + 6], v[8 * j + 7], p.aux_type));
-                            if (p.pre_tma) {
-                                send(b, &map_pre, col, row0, false);
-                            } else {
-                                __syncwarp();
-                                const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
-                                for (uint32_t r = 0; r < rows; ++r) {
-                                    if (col + lane >= p.n) continue;
-                                    const uint32_t byte = lane * 2;
-                                    static_cast<uint16_t*>(p.pre)[(row0 + r) * p.ldp + col + lane] =
-                                        *reinterpret_cast<const uint16_t*>(
-                                            b + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
-                                }
-                                __syncwarp();
-                                if (lane == 0) bulk_commit();
-                            }
+                            uint32_t w[16];
+                            pack32(v, w, p.aux_type);
+                            put_words(b, w);
                         }
+                        if (p.pre_tma)
+                            send(b, &map_pre, col, row0, false);
+                        else
+                            copy_out(b, p.pre, p.ldp, p.aux_type == kF32 ? 4 : 2, row0, col);
                     }
                     switch (p.activation) {
                         case kActRelu: act_all<kActRelu>(v); break;
@@ -704,18 +794,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                                     v[4 * j + 3] += q.w;
                                 }
                             } else {
-                                const uint4* r4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const uint4 q = r4[j];
-                                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                                    for (int h = 0; h < 4; ++h) {
-                                        const float2 f = unpack2(w[h], p.aux_type);
-                                        v[8 * j + 2 * h] += f.x;
-                                        v[8 * j + 2 * h + 1] += f.y;
-                                    }
-                                }
+                                add_words(v, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at),
+                                          p.aux_type);
                             }
                         } else {
 #pragma unroll
@@ -723,58 +803,29 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                                 if (col + j < p.n) v[j] += load_elem(p.residual, at + j, p.aux_type);
                         }
                     }
-                    if (osize == 4) {
-                        uint8_t* b = next_box();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            put(b, j, make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                 __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
-                        if (p.out_tma)
-                            send(b, &map_out, col, out_row0, p.accumulate != 0);
-                        else
-                            copy_out(b, p.out, p.ldo, 4, row0, col);
+                    uint8_t* b = next_box();
+                    if (p.out_type == kF32) {
+                        put_f32(b, v);
                     } else {
-                        uint4 now[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            now[j] = make_uint4(pack2(v[8 * j], v[8 * j + 1], p.out_type),
-                                                pack2(v[8 * j + 2], v[8 * j + 3], p.out_type),
-                                                pack2(v[8 * j + 4], v[8 * j + 5], p.out_type),
-                                                pack2(v[8 * j + 6], v[8 * j + 7], p.out_type));
-                        if ((c & 32) == 0) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) keep[j] = now[j];
-                        } else {
-                            uint8_t* b = next_box();
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                put(b, j, keep[j]);
-                                put(b, j + 4, now[j]);
-                            }
-                            if (p.out_tma)
-                                send(b, &map_out, col - 32, out_row0, false);
-                            else
-                                copy_out(b, p.out, p.ldo, 2, row0, col - 32);
-                        }
+                        uint32_t w[16];
+                        pack32(v, w, p.out_type);
+                        put_words(b, w);
                     }
-                }
+                    if (p.out_tma)
+                        send(b, &map_out, col, out_row0, p.accumulate != 0);
+                    else
+                        copy_out(b, p.out, p.ldo, p.out_type == kF32 ? 4 : 2, row0, col);
+                });
             } else if constexpr (EPI == kEpiSoftmax) {
                 // Running maximum (of the scaled logits, base 2) and sum of
                 // 2^(logit - maximum) of this row over its half of the columns,
                 // the label's column left out.
                 float top = -INFINITY, sum = 0.0f;
                 const int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
-                for (uint32_t tn = t.n0; tn < t.n1; ++tn) {
-                    uint32_t buf;
-                    ok = tile_ready(t.p1 - t.p0, buf);
-                    if (!ok) break;
-                    const uint32_t col_base = tn * BN + half * kCols;
-#pragma unroll kUnroll
-                    for (int c = 0; c < kCols; c += 32) {
-                        float v[32];
-                        load32(buf, c, v);
-                        if (c + 32 == kCols) release(buf);
-                        const uint32_t col = col_base + c;
+                for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
+                    const uint32_t col_base = tn * bn_tile + half * 32;
+                    ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
+                        const uint32_t col = col_base + i * 64;
                         const int32_t at = label - static_cast<int32_t>(col);
                         if (at >= 0 && at < 32) {
                             float z = 0.0f;
@@ -790,10 +841,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                             for (int j = 0; j < 32; ++j)
                                 if (col + j >= p.n) v[j] = -INFINITY;
                         }
-                        float big = v[0];
+                        float big[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                        for (int j = 1; j < 32; ++j) big = fmaxf(big, v[j]);
-                        const float now = fmaxf(top, big * p.scale2);
+                        for (int j = 4; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], v[j]);
+                        const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+                        const float now = fmaxf(top, most * p.scale2);
                         // A row whose logits so far are all -inf has no sum yet.
                         const float base = now == -INFINITY ? 0.0f : now;
                         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -801,87 +853,62 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(v[j], p.scale2, -base));
                         sum = sum * exp2_approx(top - base) + ((part[0] + part[1]) + (part[2] + part[3]));
                         top = now;
-                    }
+                    });
                 }
                 if (ok && live) p.part[uint64_t(2 * t.segment + half) * p.m + row] = make_float2(top, sum);
             } else {
                 const float lse2 = live ? p.lse2[row] : 0.0f;
-                float cmax_inv = 1.0f;
-                if (p.alpha_dev) cmax_inv = *p.alpha_dev > 0.0f ? 1.0f / *p.alpha_dev : 0.0f;
+                const float cmax_inv = *p.alpha_dev > 0.0f ? 1.0f / *p.alpha_dev : 0.0f;
                 const float coef = live ? p.coef[row] * cmax_inv * p.grad_scale : 0.0f;
                 // Column of the row's class here; negative where it has none or an earlier piece holds it.
                 int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
                 if (label >= 0) label -= static_cast<int32_t>(p.class0);
-                uint32_t buf;
-                ok = tile_ready(t.p1 - t.p0, buf);
-                if (!ok) break;
-                const uint32_t col_base = t.n0 * BN + half * kCols;
-#pragma unroll kUnroll2
-                for (int c = 0; c < kCols; c += 64) {
-                    uint4 lo[8], mid[8], low[8];
-                    const uint32_t col0 = col_base + c;
+                const uint32_t col_base = t.n0 * bn_tile + half * 32;
+                // Planes are read in whole K blocks of 64 columns.
+                const uint32_t width = p.grad_planes == 1 ? p.n : (p.n + 63) / 64 * 64;
+                ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
+                    const uint32_t col = col_base + i * 64;
+                    if (row0 >= p.m || col >= width) return;
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        float v[32];
-                        load32(buf, c + 32 * hh, v);
-                        if (c + 32 * hh + 32 == kCols) release(buf);
-                        const uint32_t col = col0 + 32 * hh;
+                    for (int j = 0; j < 32; ++j) v[j] = coef * exp2_approx(fmaf(v[j], p.scale2, -lse2));
+                    const int32_t at = label - static_cast<int32_t>(col);
+                    if (at >= 0 && at < 32) {
+                        float g = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = coef * exp2_approx(fmaf(v[j], p.scale2, -lse2));
-                        const int32_t at = label - static_cast<int32_t>(col);
-                        if (at >= 0 && at < 32) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j == at) v[j] -= coef;
+                        for (int j = 0; j < 32; ++j) {
+                            if (j == at) g = v[j] -= coef;
                         }
-                        if (p.grad_planes == 3 && col + 32 > p.n) {  // pad columns of a plane hold zeros
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (col + j >= p.n) v[j] = 0.0f;
+                        if (p.grad_planes == 1 && col + at < p.n) {
+                            const uint32_t w = pack2(g, 0.0f, p.in_type);
+                            p.label_rest[row] = g - unpack2(w, p.in_type).x;
                         }
-                        uint32_t w[16];
+                    }
+                    if (col + 32 > p.n) {  // pad columns hold zeros
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], p.in_type);
+                        for (int j = 0; j < 32; ++j)
+                            if (col + j >= p.n) v[j] = 0.0f;
+                    }
+                    uint32_t w[16];
+                    pack32(v, w, p.in_type);
+                    uint8_t* b = next_box();
+                    put_words(b, w);
+                    send(b, &map_out, col, row0, false);
+                    if (p.grad_planes == 3) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            lo[4 * hh + j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-                        if (p.grad_planes == 3) {
-                            uint32_t wm[16], wl[16];
+                        for (int plane = 1; plane < 3; ++plane) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                float2 f = unpack2(w[j], kBF16);
-                                const float r0 = v[2 * j] - f.x, r1 = v[2 * j + 1] - f.y;
-                                wm[j] = pack2(r0, r1, kBF16);
-                                f = unpack2(wm[j], kBF16);
-                                wl[j] = pack2(r0 - f.x, r1 - f.y, kBF16);
+                                const float2 f = unpack2(w[j], kBF16);
+                                v[2 * j] -= f.x;
+                                v[2 * j + 1] -= f.y;
                             }
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                mid[4 * hh + j] = make_uint4(wm[4 * j], wm[4 * j + 1], wm[4 * j + 2], wm[4 * j + 3]);
-                                low[4 * hh + j] = make_uint4(wl[4 * j], wl[4 * j + 1], wl[4 * j + 2], wl[4 * j + 3]);
-                            }
+                            pack32(v, w, kBF16);
+                            b = next_box();
+                            put_words(b, w);
+                            send(b, &map_out, plane * p.grad_pitch + col, row0, false);
                         }
                     }
-                    if (p.grad_planes == 1) {
-                        uint8_t* b = next_box();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) put(b, j, lo[j]);
-                        send(b, &map_out, col0, row0, false);
-                    } else if (col0 < p.grad_pitch) {
-                        uint8_t* b = next_box();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) put(b, j, lo[j]);
-                        send(b, &map_out, col0, row0, false);
-                        b = next_box();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) put(b, j, mid[j]);
-                        send(b, &map_out, p.grad_pitch + col0, row0, false);
-                        b = next_box();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) put(b, j, low[j]);
-                        send(b, &map_out, 2 * p.grad_pitch + col0, row0, false);
-                    }
-                }
+                });
             }
         }
         if (!ok && lane == 0) abort_all();
