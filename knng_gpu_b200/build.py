@@ -38,7 +38,7 @@ def build_gpu(verbose: bool = False, force: bool = False) -> Path:
     units = {
         "knng_gpu.cu": ["internal.hpp", "knn_exact.cuh", "knn_pair.cuh", "knn_rerank.cuh", "knn_tc.cuh", "ptx.cuh",
                         "schedule.cuh", "sharded.cuh", "topk.cuh"],
-        "learn.cu": ["internal.hpp", "learn.cuh", "product.cuh", "ptx.cuh"],
+        "learn.cu": ["internal.hpp", "learn.cuh", "product.cuh", "ptx.cuh", "skinny.cuh"],
     }
     sources = {name: [CSRC / name, *(CSRC / p for p in parts), ROOT / "include" / "knng_gpu.h"]
                for name, parts in units.items()}
