@@ -30,9 +30,14 @@ from .api import (  # noqa: F401
     recall_at_k,
     workspace_bytes,
 )
-from .learn import (  # noqa: F401
-    linear,
-    linear_backward,
-    softmax_xent,
-    softmax_xent_backward,
-)
+
+_LEARN = ("linear", "linear_backward", "softmax_xent", "softmax_xent_backward")
+
+
+def __getattr__(name: str):
+    # The torch operators, loaded on first use: the rest of the package works without torch.
+    if name in _LEARN:
+        from . import learn
+
+        return getattr(learn, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

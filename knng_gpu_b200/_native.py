@@ -201,10 +201,10 @@ def gpu_lib() -> ctypes.CDLL:
                  c_uint64, c_void_p, st],
             ),
         }
-        for name, args in (("linear", LinearArgs), ("linear_backward", LinearBackwardArgs),
-                           ("softmax_xent", SoftmaxXentArgs), ("softmax_xent_backward", SoftmaxXentBackwardArgs)):
-            sig[f"knng_gpu_{name}_workspace_bytes"] = (c_uint64, [POINTER(args)])
-            sig[f"knng_gpu_{name}"] = (c_int, [POINTER(args), c_void_p, c_uint64, c_void_p])
+        # The argument structures go by address (byref) or as the same bytes.
+        for name in ("linear", "linear_backward", "softmax_xent", "softmax_xent_backward"):
+            sig[f"knng_gpu_{name}_workspace_bytes"] = (c_uint64, [c_void_p])
+            sig[f"knng_gpu_{name}"] = (c_int, [c_void_p, c_void_p, c_uint64, c_void_p])
         del f32p, u32p, i32p
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)

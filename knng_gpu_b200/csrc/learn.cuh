@@ -11,12 +11,16 @@ namespace knng_b200 {
 // can read, 3 splits fp32 values into bf16 parts x = h + m + l (each rounded to
 // nearest from what is left; a finite value whose rounding would overflow is
 // truncated). Columns past k are zeros. Rows without a label are zeros when
-// labels are given. One thread per 8 columns.
+// labels are given. One thread per 8 columns. Also clears *zero, if given, for
+// the kernel after it.
 template <int PLANES>
 __global__ void __launch_bounds__(256) stage_rows_kernel(const void* __restrict__ x, uint64_t rows, uint32_t k,
                                                          uint64_t ld, uint16_t* __restrict__ out, uint32_t pitch,
-                                                         const void* labels, int labels_i64, uint32_t classes)
+                                                         const void* labels, int labels_i64, uint32_t classes,
+                                                         float* zero)
 {
+    previous_done();
+    if (zero && blockIdx.x == 0 && threadIdx.x == 0) *zero = 0.0f;
     const uint32_t groups = pitch / 8;
     const uint64_t total = rows * groups;
     for (uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
@@ -106,6 +110,7 @@ struct JoinParams {
 // The pieces of a split product, summed in order, and the linear epilogue.
 __global__ void __launch_bounds__(256) join_splits_kernel(const JoinParams p)
 {
+    previous_done();
     const uint32_t groups = (p.n + 3) / 4;
     const uint64_t total = p.m * groups;
     const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
@@ -147,31 +152,40 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const JoinParams p)
 //   loss = log(1 + S 2^(M - y)), lse = y ln 2 + loss        where y >= M,
 //   loss = (M - y) ln 2 + log(S + 2^(y - M)), lse likewise  where it is not.
 // So the small loss of a well placed row keeps its digits. Without a label
-// lse = M ln 2 + log S. One warp per row.
+// lse = M ln 2 + log S. LANES threads per row: a warp, or a block.
+template <int LANES>
 __global__ void __launch_bounds__(256) join_softmax_kernel(const float2* __restrict__ part, uint32_t pieces,
                                                            uint64_t m, const float* __restrict__ label_dot,
                                                            float scale2, const void* labels, int labels_i64,
                                                            uint32_t classes, float* __restrict__ loss,
                                                            float* __restrict__ lse)
 {
-    const uint64_t r = blockIdx.x * uint64_t(8) + (threadIdx.x >> 5);
+    __shared__ float2 warps[8];
+    previous_done();
+    const uint64_t r = blockIdx.x * uint64_t(256 / LANES) + threadIdx.x / LANES;
     const int lane = threadIdx.x & 31;
     if (r >= m) return;
     float top = -INFINITY, sum = 0.0f;
-    for (uint32_t s = lane; s < pieces; s += 32) {
-        const float2 q = part[uint64_t(s) * m + r];
-        const float now = fmaxf(top, q.x);
-        const float base = now == -INFINITY ? 0.0f : now;
-        sum = sum * exp2_approx(top - base) + q.y * exp2_approx(q.x - base);
-        top = now;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float t2 = __shfl_xor_sync(~0u, top, o), s2 = __shfl_xor_sync(~0u, sum, o);
+    const auto merge = [&](float t2, float s2) {
         const float now = fmaxf(top, t2);
         const float base = now == -INFINITY ? 0.0f : now;
         sum = sum * exp2_approx(top - base) + s2 * exp2_approx(t2 - base);
         top = now;
+    };
+    for (uint32_t s = threadIdx.x % LANES; s < pieces; s += LANES) {
+        const float2 q = part[uint64_t(s) * m + r];
+        merge(q.x, q.y);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const float t2 = __shfl_xor_sync(~0u, top, o), s2 = __shfl_xor_sync(~0u, sum, o);
+        merge(t2, s2);
+    }
+    if constexpr (LANES > 32) {  // the row is the block's: no thread has left
+        if (lane == 0) warps[threadIdx.x >> 5] = make_float2(top, sum);
+        __syncthreads();
+        if (threadIdx.x != 0) return;
+        for (int w = 1; w < 8; ++w) merge(warps[w].x, warps[w].y);
     }
     if (lane == 0) {
         const bool has = load_label(labels, labels_i64, r, classes) >= 0;
@@ -201,6 +215,7 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
                                                         uint32_t classes, float* __restrict__ coef,
                                                         float* __restrict__ lse2, uint32_t* cmax)
 {
+    previous_done();
     float big = 0.0f;
     for (uint64_t r = blockIdx.x * uint64_t(256) + threadIdx.x; r < m; r += uint64_t(gridDim.x) * 256) {
         const bool has = load_label(labels, labels_i64, r, classes) >= 0;
@@ -260,6 +275,7 @@ template <int ACT, int TYPE>
 __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
 {
     __shared__ float total[8][256];
+    previous_done();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t c0 = blockIdx.x * 256 + lane * 8;
     const uint64_t r0 = p.m * blockIdx.y / gridDim.y, r1 = p.m * (blockIdx.y + 1) / gridDim.y;
@@ -319,6 +335,7 @@ __global__ void __launch_bounds__(256) join_sums_kernel(const float* __restrict_
                                                         void* out, int type)
 {
     __shared__ float part[8][32];
+    previous_done();
     const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t c = blockIdx.x * 32 + lane;
     float s = 0.0f;

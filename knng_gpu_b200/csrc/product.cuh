@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    previous_done();
 
     auto abort_all = [&]() {
         *p.error = 1;

@@ -323,6 +323,15 @@ __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t nthread
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// For kernels launched with programmatic stream serialization: waits until the
+// kernels before this one in the stream are done and their writes visible, then
+// lets the next one be set up. Without that launch attribute it does nothing.
+__device__ __forceinline__ void previous_done()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+}
+
 // ---------------------------------------------------------------- CTA pairs (cluster of 2)
 // Rank of this CTA in its cluster.
 __device__ __forceinline__ uint32_t cluster_ctarank()

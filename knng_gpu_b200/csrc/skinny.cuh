@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
 
+    previous_done();
+
     // x into shared memory, 8 values a thread at a time, zeros past its rows
     // and columns.
     const uint32_t octets = p.pitch / (4 * kWords);

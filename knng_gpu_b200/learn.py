@@ -18,88 +18,132 @@ C ABI's), allocated here when not given. The operators build no autograd graph.
 """
 from __future__ import annotations
 
-import ctypes
 from contextlib import nullcontext
+from struct import Struct
 
-from . import _native
+import torch
+
 from ._native import gpu_lib
 from .api import InvalidArgument, check
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-_dtypes: dict = {}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_current_scope = nullcontext()
+
+
+class _Operator:
+    """One C entry point: its argument structure as a byte format (the mirrors
+    in _native spell the fields out), its two functions once loaded."""
+
+    def __init__(self, name: str, fields: str):
+        self.name, self.fields = name, Struct(fields)
+        self.size = self.call = None
+
+    def run(self, device, workspace, *values) -> None:
+        """On the current device and stream of the caller's :func:`_scope`."""
+        if self.call is None:
+            lib = gpu_lib()
+            self.size = getattr(lib, f"knng_gpu_{self.name}_workspace_bytes")
+            self.call = getattr(lib, f"knng_gpu_{self.name}")
+        args = self.fields.pack(*values)
+        if workspace is None:
+            need = self.size(args)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
+        if workspace is None:
+            status = self.call(args, None, 0, stream)
+        else:
+            status = self.call(args, workspace.data_ptr(), workspace.numel(), stream)
+        if status:
+            check(status)
+
+
+# The current stream's handle without making a Stream object (2 us), where torch offers it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+_LINEAR = _Operator("linear", "14Q3i4x")
+_LINEAR_BACKWARD = _Operator("linear_backward", "14Q2i")
+_XENT = _Operator("softmax_xent", "10Qf2i4x")
+_XENT_BACKWARD = _Operator("softmax_xent_backward", "12Qf2i4x")
 
 
 def _dtype_id(op: str, dtype) -> int:
-    if not _dtypes:
-        import torch
-
-        _dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    if dtype not in _dtypes:
+    d = _DTYPES.get(dtype)
+    if d is None:
         raise InvalidArgument(f"knng::gpu::{op}: dtype must be float32, bfloat16 or float16, not {dtype}")
-    return _dtypes[dtype]
+    return d
 
 
-def _matrix(op: str, name: str, t, rows: int | None, cols: int | None, like=None):
-    """Row stride of a 2-D tensor after its checks (None sizes are free)."""
+def _stride(op: str, name: str, t, rows: int, cols: int) -> int:
+    """Row stride of a 2-D CUDA tensor of that shape, after its checks."""
     if t.dim() != 2 or not t.is_cuda:
         raise InvalidArgument(f"knng::gpu::{op}: {name} must be a 2-D CUDA tensor")
-    r, c = t.shape
-    if (rows is not None and r != rows) or (cols is not None and c != cols):
-        raise InvalidArgument(f"knng::gpu::{op}: {name} is {tuple(t.shape)}, expected "
-                              f"({'any' if rows is None else rows}, {'any' if cols is None else cols})")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise InvalidArgument(f"knng::gpu::{op}: {name} must have the dtype and device of the other operands")
+    if t.shape != (rows, cols):
+        raise InvalidArgument(f"knng::gpu::{op}: {name} is {tuple(t.shape)}, expected ({rows}, {cols})")
     s0, s1 = t.stride()
-    if c > 1 and s1 != 1:
+    if s1 != 1 and cols > 1:
         raise InvalidArgument(f"knng::gpu::{op}: the rows of {name} must be contiguous")
-    if r <= 1:
-        return c
-    if s0 < c:
+    if rows <= 1:
+        return cols
+    if s0 < cols:
         raise InvalidArgument(f"knng::gpu::{op}: the rows of {name} overlap")
     return s0
 
 
-def _vector(op: str, name: str, t, n: int, dtype, device):
+def _operands(op: str, x, w):
+    """Sizes, strides and type of x (m, k) and w (n, k)."""
+    if x.dim() != 2 or w.dim() != 2:
+        raise InvalidArgument(f"knng::gpu::{op}: x and w must be 2-D CUDA tensors")
+    m, k = x.shape
+    n = w.shape[0]
+    _same(op, "w", w, x)
+    return m, k, n, _stride(op, "x", x, m, k), _stride(op, "w", w, n, k), _dtype_id(op, x.dtype)
+
+
+def _same(op: str, name: str, t, x) -> None:
+    if t.dtype != x.dtype or t.device != x.device:
+        raise InvalidArgument(f"knng::gpu::{op}: {name} must have the dtype and device of x")
+
+
+def _vector(op: str, name: str, t, n: int, dtype, device) -> int:
+    """Address of a dense vector."""
     if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or t.device != device:
         raise InvalidArgument(f"knng::gpu::{op}: {name} must be a {dtype} vector of {n} values on {device}")
     if n > 1 and t.stride(0) != 1:
         raise InvalidArgument(f"knng::gpu::{op}: {name} must be contiguous")
+    return t.data_ptr()
 
 
-def _labels(op: str, t, m: int, device) -> int:
-    import torch
-
+def _labels(op: str, t, m: int, device):
+    """Address and whether int64."""
     if t.dtype not in (torch.int64, torch.int32):
         raise InvalidArgument(f"knng::gpu::{op}: labels must be int64 or int32")
-    _vector(op, "labels", t, m, t.dtype, device)
-    return int(t.dtype == torch.int64)
+    return _vector(op, "labels", t, m, t.dtype, device), int(t.dtype == torch.int64)
+
+
+def _activation(op: str, name: str) -> int:
+    act = ACTIVATIONS.get(name)
+    if act is None:
+        raise InvalidArgument(f"knng::gpu::{op}: unknown activation {name!r}")
+    return act
 
 
 def _scope(device, stream):
     """Allocations and launches on the tensors' device and the call's stream."""
-    import torch
-
     if stream is not None:
         return torch.cuda.stream(stream)
-    if device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch.cuda.current_device():
         return torch.cuda.device(device)
-    return nullcontext()
+    return _current_scope
 
 
-def _run(name: str, args, device, workspace) -> None:
-    """Inside :func:`_scope`."""
-    import torch
+def _rows(rows: int, cols: int, dtype, device):
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
-    lib = gpu_lib()
-    ref = ctypes.byref(args)
-    ws, have = None, 0
-    if workspace is None:
-        need = getattr(lib, f"knng_gpu_{name}_workspace_bytes")(ref)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    if workspace is not None:
-        ws, have = workspace.data_ptr(), workspace.numel()
-    check(getattr(lib, f"knng_gpu_{name}")(ref, ws, have, torch.cuda.current_stream(device).cuda_stream))
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def linear(x, w, bias=None, residual=None, activation="none", out_dtype=None, out=None, save_pre=False,
@@ -111,37 +155,26 @@ def linear(x, w, bias=None, residual=None, activation="none", out_dtype=None, ou
     instead of x's. With ``save_pre`` returns ``(out, pre)``, pre = x w^T +
     bias in x's dtype, which :func:`linear_backward` takes.
     """
-    import torch
-
     op = "linear"
-    dtype = _dtype_id(op, x.dtype)
-    ldx = _matrix(op, "x", x, None, None)
-    m, k = x.shape
-    ldw = _matrix(op, "w", w, None, k, x)
-    n = w.shape[0]
-    if activation not in ACTIVATIONS:
-        raise InvalidArgument(f"knng::gpu::linear: unknown activation {activation!r}")
+    m, k, n, ldx, ldw, dtype = _operands(op, x, w)
+    act = _activation(op, activation)
     device = x.device
     ldr = 0
     if bias is not None:
         _vector(op, "bias", bias, n, x.dtype, device)
     if residual is not None:
-        ldr = _matrix(op, "residual", residual, m, n, x)
-    if out is not None:
-        if out_dtype is not None and out.dtype != out_dtype:
-            raise InvalidArgument("knng::gpu::linear: out has another dtype than out_dtype")
-        if out.device != device:
-            raise InvalidArgument("knng::gpu::linear: out is on another device")
-        _matrix(op, "out", out, m, n)
+        _same(op, "residual", residual, x)
+        ldr = _stride(op, "residual", residual, m, n)
+    if out is not None and (out.device != device or (out_dtype is not None and out.dtype != out_dtype)):
+        raise InvalidArgument("knng::gpu::linear: out has another dtype or device than asked for")
     with _scope(device, stream):
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype or x.dtype, device=device)
-        pre = torch.empty((m, n), dtype=x.dtype, device=device) if save_pre else None
-        args = _native.LinearArgs(
-            m, k, n, x.data_ptr(), ldx, w.data_ptr(), ldw, None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), _matrix(op, "out", out, m, n),
-            None if pre is None else pre.data_ptr(), n, dtype, _dtype_id(op, out.dtype), ACTIVATIONS[activation])
-        _run(op, args, device, workspace)
+            out, ldo = _rows(m, n, out_dtype or x.dtype, device), n
+        else:
+            ldo = _stride(op, "out", out, m, n)
+        pre = _rows(m, n, x.dtype, device) if save_pre else None
+        _LINEAR.run(device, workspace, m, k, n, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr,
+                    out.data_ptr(), ldo, _ptr(pre), n, dtype, _dtype_id(op, out.dtype), act)
     return (out, pre) if save_pre else out
 
 
@@ -150,33 +183,23 @@ def linear_backward(dy, x, w, pre=None, activation="none", need_dx=True, need_dw
     """Gradients of :func:`linear` from ``dy`` (m, n): ``(dx, dw, db)``, None
     where not needed. ``pre`` is what the forward call saved (not needed
     without an activation). The residual's gradient is ``dy``."""
-    import torch
-
     op = "linear_backward"
-    dtype = _dtype_id(op, x.dtype)
-    ldx = _matrix(op, "x", x, None, None)
-    m, k = x.shape
-    ldw = _matrix(op, "w", w, None, k, x)
-    n = w.shape[0]
-    lddy = _matrix(op, "dy", dy, m, n, x)
-    if activation not in ACTIVATIONS:
-        raise InvalidArgument(f"knng::gpu::linear_backward: unknown activation {activation!r}")
-    ldp = 0
+    m, k, n, ldx, ldw, dtype = _operands(op, x, w)
+    act = _activation(op, activation)
+    _same(op, "dy", dy, x)
+    lddy, ldp = _stride(op, "dy", dy, m, n), 0
     if pre is not None:
-        ldp = _matrix(op, "pre", pre, m, n, x)
-    elif activation != "none":
+        _same(op, "pre", pre, x)
+        ldp = _stride(op, "pre", pre, m, n)
+    elif act:
         raise InvalidArgument("knng::gpu::linear_backward: pre is needed with an activation")
     device = x.device
     with _scope(device, stream):
-        dx = torch.empty((m, k), dtype=x.dtype, device=device) if need_dx else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=device) if need_dw else None
+        dx = _rows(m, k, x.dtype, device) if need_dx else None
+        dw = _rows(n, k, x.dtype, device) if need_dw else None
         db = torch.empty(n, dtype=x.dtype, device=device) if need_db else None
-        args = _native.LinearBackwardArgs(
-            m, k, n, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw,
-            None if pre is None else pre.data_ptr(), ldp, None if dx is None else dx.data_ptr(),
-            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), dtype,
-            ACTIVATIONS[activation])
-        _run(op, args, device, workspace)
+        _LINEAR_BACKWARD.run(device, workspace, m, k, n, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw,
+                             _ptr(pre), ldp, _ptr(dx), _ptr(dw), _ptr(db), dtype, act)
     return dx, dw, db
 
 
@@ -184,21 +207,15 @@ def softmax_xent(x, w, labels, scale=1.0, workspace=None, stream=None):
     """Per-row softmax cross entropy over ``scale * x w^T``: ``(loss, lse)``,
     float32 (m,). ``labels`` (m,) int64 or int32 name a row of w; a label
     outside [0, n) leaves its row out (loss 0; lse is still that row's)."""
-    import torch
-
     op = "softmax_xent"
-    dtype = _dtype_id(op, x.dtype)
-    ldx = _matrix(op, "x", x, None, None)
-    m, k = x.shape
-    ldw = _matrix(op, "w", w, None, k, x)
+    m, k, n, ldx, ldw, dtype = _operands(op, x, w)
     device = x.device
-    i64 = _labels(op, labels, m, device)
+    y, i64 = _labels(op, labels, m, device)
     with _scope(device, stream):
-        loss = torch.empty(m, dtype=torch.float32, device=device)
-        lse = torch.empty(m, dtype=torch.float32, device=device)
-        args = _native.SoftmaxXentArgs(m, k, w.shape[0], x.data_ptr(), ldx, w.data_ptr(), ldw, labels.data_ptr(),
-                                       loss.data_ptr(), lse.data_ptr(), scale, dtype, i64)
-        _run(op, args, device, workspace)
+        loss = torch.empty_strided((m,), (1,), dtype=torch.float32, device=device)
+        lse = torch.empty_strided((m,), (1,), dtype=torch.float32, device=device)
+        _XENT.run(device, workspace, m, k, n, x.data_ptr(), ldx, w.data_ptr(), ldw, y, loss.data_ptr(), lse.data_ptr(),
+                  scale, dtype, i64)
     return loss, lse
 
 
@@ -207,23 +224,15 @@ def softmax_xent_backward(dloss, x, w, labels, lse, scale=1.0, need_dx=True, nee
     """Gradients of :func:`softmax_xent` from ``dloss`` (m,) float32 and the
     forward call's ``lse``: ``(dx, dw)`` in x's dtype, None where not needed.
     A row without a label has dx 0 and adds nothing to dw, whatever it holds."""
-    import torch
-
     op = "softmax_xent_backward"
-    dtype = _dtype_id(op, x.dtype)
-    ldx = _matrix(op, "x", x, None, None)
-    m, k = x.shape
-    ldw = _matrix(op, "w", w, None, k, x)
-    n = w.shape[0]
+    m, k, n, ldx, ldw, dtype = _operands(op, x, w)
     device = x.device
-    i64 = _labels(op, labels, m, device)
-    _vector(op, "dloss", dloss, m, torch.float32, device)
-    _vector(op, "lse", lse, m, torch.float32, device)
+    y, i64 = _labels(op, labels, m, device)
+    at_dloss = _vector(op, "dloss", dloss, m, torch.float32, device)
+    at_lse = _vector(op, "lse", lse, m, torch.float32, device)
     with _scope(device, stream):
-        dx = torch.empty((m, k), dtype=x.dtype, device=device) if need_dx else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=device) if need_dw else None
-        args = _native.SoftmaxXentBackwardArgs(
-            m, k, n, dloss.data_ptr(), x.data_ptr(), ldx, w.data_ptr(), ldw, labels.data_ptr(), lse.data_ptr(),
-            None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), scale, dtype, i64)
-        _run(op, args, device, workspace)
+        dx = _rows(m, k, x.dtype, device) if need_dx else None
+        dw = _rows(n, k, x.dtype, device) if need_dw else None
+        _XENT_BACKWARD.run(device, workspace, m, k, n, at_dloss, x.data_ptr(), ldx, w.data_ptr(), ldw, y, at_lse,
+                           _ptr(dx), _ptr(dw), scale, dtype, i64)
     return dx, dw

@@ -169,3 +169,12 @@ def test_definitions_agree_with_autograd():
     (dx, _), (dw, _) = xent_backward64(dloss, x, w, labels, lse, 2.5)
     # lse reaches the gradient in fp32 in use; here it is the 64-bit one.
     assert torch.allclose(dx, xd.grad, atol=1e-12) and torch.allclose(dw, wd.grad, atol=1e-12)
+
+
+def test_argument_formats_match_the_structures():
+    from knng_gpu_b200 import learn
+
+    for op, args in ((learn._LINEAR, _native.LinearArgs), (learn._LINEAR_BACKWARD, _native.LinearBackwardArgs),
+                     (learn._XENT, _native.SoftmaxXentArgs), (learn._XENT_BACKWARD, _native.SoftmaxXentBackwardArgs)):
+        values = [1.5 if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(args._fields_)]
+        assert op.fields.pack(*values) == bytes(args(*values)), op.name
