@@ -222,14 +222,17 @@ struct Shape {
     uint64_t m, n, k;
     uint32_t combos;
     bool precise;  // the result is kept in fp32
+    bool bf16;     // operands are single bf16 values
 };
 
-// Longest K summed by the tensor cores alone (their additions truncate): 128
-// where fp32 comes of it, 1024 where 16 bits do. Against 64 bits, lse of fp16
-// rows of width 785 is off by 1.9e-6 of its size when K is summed in one
-// piece and by 1.9e-7 in pieces of 128 (plain fp32: 0.8e-7); a 16-bit result
-// has 2e-4 or more of its own.
-constexpr uint32_t kPreciseBlocks = 2, kShortBlocks = 16;
+// K blocks of 64 summed by the tensor cores alone, whose additions truncate:
+// 1024 of K where 16 bits come of it, 256 (bf16) or 128 (fp16, whose products
+// are longer, and fp32) where the result stays fp32. Loss of 2048 rows of
+// width 960 against 30,000, relative error against 64 bits: bf16 1.3e-6 at 128,
+// 2.4e-6 at 256 (and 1046 us instead of 1257 for 8192 rows against 100,000);
+// fp16 2.3e-6 and 5.5e-6; plain fp32 3.6e-6 and 4.4e-6. A 16-bit result has
+// 2e-4 or more of its own.
+uint32_t piece_blocks(const Shape& s) { return !s.precise ? 16u : s.bf16 ? 4u : 2u; }
 
 struct Plan {
     int cg;
@@ -248,7 +251,7 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
     q.tiles_n = static_cast<uint32_t>(ceil_div(s.n, tile_n));
     q.kblocks = static_cast<uint32_t>(ceil_div(s.k, 64));
     q.splits = 1;
-    q.piece = std::min(q.kblocks, s.precise ? kPreciseBlocks : kShortBlocks);
+    q.piece = std::min(q.kblocks, piece_blocks(s));
     q.split_rows = uint64_t(q.tiles_m) * 128 * cg;
     q.part_pitch = uint64_t(q.tiles_n) * tile_n;
     return q;
@@ -334,13 +337,21 @@ knng_gpu_status launch_product_t(const CUtensorMap& a, const CUtensorMap& b, con
     at[0].val.clusterDim.x = CG;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kPkThreads);
+    cfg.blockDim = dim3(pk_threads(CG, EPI, LONG));
     cfg.dynamicSmemBytes = kPkSmem;
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     KNNG_TRY(allow_smem<kern>(kPkSmem));
     if (units == 0) {
+        // The kernel's roles trade registers within what the launch gives them.
+        constexpr int kWarps = pk_epi_warps(CG, EPI, LONG);
+        static_assert(4 * kPkIssueRegs + kWarps * pk_epi_regs(kWarps) <= (4 + kWarps) * pk_launch_regs(kWarps),
+                      "register split");
+        cudaFuncAttributes fa;
+        KNNG_CUDA(cudaFuncGetAttributes(&fa, kern));
+        if (fa.numRegs < pk_launch_regs(kWarps))
+            return fail(KNNG_GPU_CUDA_ERROR, "knng::gpu: product kernel built with too few registers");
         units = sm_count() / CG;
         if (CG == 2) {
             int clusters = 0;
@@ -616,7 +627,8 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     if (need) *need = 0;
     if (a.m == 0) return KNNG_GPU_OK;
     const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
-    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, a.out_dtype == KNNG_DTYPE_F32};
+    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, a.out_dtype == KNNG_DTYPE_F32,
+                  a.dtype == KNNG_DTYPE_BF16};
     const bool skinny = is_skinny(a.m, a.k, a.dtype);
     const Plan q = skinny ? Plan{} : plan_product(s);
     if (skinny && need) return KNNG_GPU_OK;
@@ -710,14 +722,14 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
     const bool products = a.dx || a.dw;
     // dz lies in the workspace unless it is dy and TMA can read that.
     const bool make_dz = products && (slope || needs_stage(dy, a.dtype));
-    const Shape sx{a.m, a.k, a.n, combos, f32}, sw{a.n, a.k, a.m, combos, f32};
+    const Shape sx{a.m, a.k, a.n, combos, f32, a.dtype == KNNG_DTYPE_BF16}, sw{a.n, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16};
     const Plan qx = plan_product(sx), qw = plan_product(sw);
     KNNG_TRY(check_items(op, qx));
     KNNG_TRY(check_items(op, qw));
     const uint64_t pitch = stage_pitch(a.n, a.dtype);
     const uint32_t gx = static_cast<uint32_t>(ceil_div(pitch, 256));
     const uint32_t gy = static_cast<uint32_t>(std::max<uint64_t>(
-        1, std::min<uint64_t>({ceil_div(148 * 8, gx), ceil_div(a.m, 8), 65535})));
+        1, std::min<uint64_t>(sm_count() * uint64_t(kSlopeBlocks) / gx, ceil_div(a.m, 8))));
     Carver c(ws);
     uint16_t* dz = make_dz ? c.take<uint16_t>(a.m * pitch * planes_of(a.dtype)) : nullptr;
     uint16_t* xs = a.dw && needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
@@ -749,7 +761,6 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
         p.n = static_cast<uint32_t>(a.n);
         p.out = dz;
         p.pitch = static_cast<uint32_t>(pitch);
-        p.planes = planes_of(a.dtype);
         p.sums = sums;
         p.vec = tma_rows(a.dy, a.lddy, e) && (!slope || tma_rows(a.pre, a.ldp, e));
         KNNG_TRY(launch_slope(p, a.activation, a.dtype, dim3(gx, gy), st));
@@ -815,7 +826,7 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     if (need) *need = 0;
     if (a.m == 0) return KNNG_GPU_OK;
     const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
-    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, true};
+    const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, true, a.dtype == KNNG_DTYPE_BF16};
     // Pairs unless they would leave SMs idle; then the columns are cut so that
     // (row tile, piece) items fill the units in whole rounds.
     const bool skinny = is_skinny(a.m, a.k, a.dtype);
@@ -824,7 +835,8 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     if (s.m <= 128 || uint64_t(q.tiles_m) * q.tiles_n < sm_count() / 2) q = tiles_of(s, 1, 128);
     KNNG_TRY(check_items(op, q));
     const uint32_t segments = softmax_segments(q);
-    const uint32_t pieces = skinny ? sq.blocks : 2 * segments;
+    const uint32_t groups = pk_epi_warps(q.cg, kEpiSoftmax, q.pieces() > 1) / 4;
+    const uint32_t pieces = skinny ? sq.blocks : groups * segments;
     Carver c(ws);
     uint16_t* xs = !skinny && needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
     uint16_t* wst = !skinny && needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
@@ -901,11 +913,11 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     const uint64_t width = up(ceil_div(a.n, pieces), 256);
     const uint64_t gpitch = up(std::min(width, a.n), 64);
     const bool f32 = planes == 3;
-    const Shape sg{a.m, std::min(width, a.n), a.k, combos, f32};
-    const Shape sx{a.m, a.k, std::min(width, a.n), combos, f32};
+    const Shape sg{a.m, std::min(width, a.n), a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
+    const Shape sx{a.m, a.k, std::min(width, a.n), combos, f32, a.dtype == KNNG_DTYPE_BF16};
     const Plan qx = plan_product(sx);
     const uint64_t xpart_rows = qx.split_rows, xpart_pitch = qx.part_pitch;
-    const auto dw_shape = [&](uint64_t cols) { return Shape{cols, a.k, a.m, combos, f32}; };
+    const auto dw_shape = [&](uint64_t cols) { return Shape{cols, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16}; };
     const uint64_t last = a.n - (ceil_div(a.n, width) - 1) * width;
     const Plan qw0 = plan_product(dw_shape(std::min(width, a.n))), qw1 = plan_product(dw_shape(last));
     for (const Plan& q : {tiles_of(sg, 1, 128), qx, qw0, qw1}) KNNG_TRY(check_items(op, q));
@@ -947,7 +959,7 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     for (uint64_t c0 = 0; c0 < a.n; c0 += width) {
         const uint64_t cols = std::min(width, a.n - c0);
         const Operand wp{static_cast<const uint16_t*>(ow.ptr) + c0 * ow.ld, cols, ow.width, ow.ld, ow.plane};
-        const Shape s1{a.m, cols, a.k, combos, f32};
+        const Shape s1{a.m, cols, a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
         Plan q1 = tiles_of(s1, 2, 256);
         if (uint64_t(q1.tiles_m) * q1.tiles_n * 2 < sm_count() * 3ull / 4) q1 = tiles_of(s1, 1, 128);
         CUtensorMap ma, mb, mo;
@@ -980,7 +992,7 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         }
         if (a.dx) {
             // Pieces add up in fp32: the first one stores, the others add.
-            const Shape sp{a.m, a.k, cols, combos, f32};
+            const Shape sp{a.m, a.k, cols, combos, f32, a.dtype == KNNG_DTYPE_BF16};
             Plan qp = qx;
             qp.kblocks = static_cast<uint32_t>(ceil_div(cols, 64));
             qp.splits = std::min(qx.splits, qp.pieces());

@@ -229,6 +229,8 @@ __global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict_
     if ((threadIdx.x & 31) == 0 && big > 0.0f) atomicMax(cmax, __float_as_uint(big));
 }
 
+constexpr int kSlopeBlocks = 4;  // per SM, all resident
+
 struct SlopeParams {
     const void* dy;
     uint64_t lddy;
@@ -238,7 +240,6 @@ struct SlopeParams {
     uint32_t n;
     uint16_t* out;        // dz as 16-bit operands (may be NULL: column sums only)
     uint32_t pitch;       // columns of a plane of out
-    uint32_t planes;
     float* sums;          // [gridDim.y][n] column sums (may be NULL)
     int vec;              // rows of dy and pre allow 16-byte loads
 };
@@ -272,7 +273,7 @@ __device__ __forceinline__ void load8(const void* p, uint64_t at, int type, uint
 // rows; its 8 warps take every eighth row, two at a time so that four 16-byte
 // loads a thread are in flight, and add up their sums in order.
 template <int ACT, int TYPE>
-__global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
+__global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopeParams p)
 {
     __shared__ float total[8][256];
     previous_done();
@@ -300,16 +301,20 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
                 acc[j] += v[h][j];
             }
             if (p.out && c0 < p.pitch) {
-                uint16_t* dst = p.out + (r + 8 * h) * (uint64_t(p.pitch) * p.planes) + c0;
                 constexpr int kOut = TYPE == kF16 ? kF16 : kBF16;
-                for (uint32_t plane = 0; plane < p.planes; ++plane) {
+                constexpr int kPlanes = TYPE == kF32 ? 3 : 1;
+                uint16_t* dst = p.out + (r + 8 * h) * (uint64_t(p.pitch) * kPlanes) + c0;
+#pragma unroll
+                for (int plane = 0; plane < kPlanes; ++plane) {
                     uint32_t w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         w[j] = pack2(v[h][2 * j], v[h][2 * j + 1], kOut);
-                        const float2 f = unpack2(w[j], kOut);
-                        v[h][2 * j] -= f.x;
-                        v[h][2 * j + 1] -= f.y;
+                        if (plane + 1 < kPlanes) {
+                            const float2 f = unpack2(w[j], kOut);
+                            v[h][2 * j] -= f.x;
+                            v[h][2 * j + 1] -= f.y;
+                        }
                     }
                     *reinterpret_cast<uint4*>(dst + plane * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
                 }

@@ -21,11 +21,10 @@
 //   warp 0      TMA producer, kStages-deep ring of 32 KiB stages
 //   warp 1      TMEM allocation; UMMA issue (leader CTA, one lane)
 //   warps 2-3   idle
-//   warps 4-11  epilogue: thread = one accumulator row; the first four warps
-//               take the even 32-column chunks of a tile, the others the odd
-//               ones, each loading a chunk from TMEM while it works on the
-//               one before. Two accumulator buffers in TMEM: the epilogue of
-//               a tile runs under the MMAs of the next one.
+//   warps 4 on  epilogue (8 or 16 warps): thread = one accumulator row, the
+//               warps of a quarter of the rows take turns with the 32-column
+//               chunks of a tile. Two accumulator buffers in TMEM: the
+//               epilogue of a tile runs under the MMAs of the next one.
 // Outputs leave through 4 KiB shared-memory boxes per warp and TMA stores
 // (reduce-adds where a call accumulates), or by coalesced element stores where
 // the output rows are not 16-byte aligned.
@@ -40,12 +39,10 @@
 
 namespace knng_b200 {
 
-constexpr int kPkThreads = 384;    // 4 + 8 warps
-constexpr int kPkEpiWarps = 8;
 constexpr int kPkStages = 5;
 constexpr int kPkStageBytes = 32768;  // 128 x 64 of A and of B, 2 bytes each
-constexpr int kPkBox = 4096;          // staging box: 32 rows x 32 columns of 4 (or 2) bytes
-constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkEpiWarps * 2 * kPkBox + 512 + 1024;
+constexpr int kPkBoxes = 65536;       // staging boxes, 32 rows x 32 columns: two per epilogue warp
+constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkBoxes + 512 + 1024;
 
 enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
@@ -87,7 +84,7 @@ struct ProductParams {
     int labels_i64;
     uint32_t classes;
     uint32_t class0;               // class of column 0
-    float2* part;                  // softmax: (max, sum) of row r, piece s, column half h at [(2 s + h) * m + r]
+    float2* part;                  // softmax: (max, sum) of row r, piece s, warp group h at [(groups s + h) * m + r]
     float* label_dot;              // softmax: x_r . w_label
     const float* lse2;             // gradient: lse * log2(e)
     const float* coef;             // gradient: dloss * scale / cmax, 0 for a row without label
@@ -152,6 +149,44 @@ __device__ __forceinline__ float exp2_approx(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pair_f32(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair_f32(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // ---------------------------------------------------------------- elementwise pieces
@@ -371,13 +406,28 @@ __device__ __forceinline__ Item decode_item(const ProductParams& p, uint32_t i)
 }
 
 // ---------------------------------------------------------------- kernel
+// Epilogue warps: 16 where a pair's tile goes through exponentials (with two
+// warps per scheduler the special-function units idle through every latency:
+// 2048 x 128 against a million rows took 621 us with 8), 8 elsewhere: long sums
+// and stores need the registers.
+__host__ __device__ constexpr int pk_epi_warps(int cg, int epi, bool longk) { return cg == 2 && epi != kEpiStore && !longk ? 16 : 8; }
+__host__ __device__ constexpr int pk_threads(int cg, int epi, bool longk) { return 128 + 32 * pk_epi_warps(cg, epi, longk); }
+// Registers a thread: what the launch gives, and the split after setmaxnreg
+// between the first warpgroup and those of the epilogue. The split never sums
+// to more than the launch gave: 56 + 2 * 224 = 3 * 168, 56 + 4 * 104 < 5 * 96.
+__host__ __device__ constexpr int pk_launch_regs(int warps) { return warps == 8 ? 168 : 96; }
+constexpr int kPkIssueRegs = 56;
+__host__ __device__ constexpr int pk_epi_regs(int warps) { return warps == 8 ? 224 : 104; }
+
 // LONG: an item may have several K pieces, whose sums are added in registers.
 template <int CG, bool AMN, bool BMN, int EPI, bool LONG>
-__global__ void __launch_bounds__(kPkThreads, 1)
+__global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
                    const ProductParams p)
 {
+    constexpr int EW = pk_epi_warps(CG, EPI, LONG);
+    constexpr int kGroups = EW / 4;          // warps that share a quarter of the rows
     constexpr uint32_t kBufCols = 128 * CG;  // TMEM columns of an accumulator buffer
     constexpr uint32_t kTmemCols = 2 * kBufCols;
     const uint32_t bn_tile = p.tile_n;
@@ -386,7 +436,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stage_base = smem;
     uint8_t* boxes = smem + kPkStages * kPkStageBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(boxes + kPkEpiWarps * 2 * kPkBox);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(boxes + kPkBoxes);
     uint64_t* full = bars;        // [kPkStages] leader: bytes of both CTAs landed
     uint64_t* empty = bars + 8;   // [kPkStages] both: MMAs that read the stage are done
     uint64_t* tfull = bars + 16;  // [2] both: accumulator ready
@@ -408,7 +458,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], CG * kPkEpiWarps);
+            mbar_init(&tempty[b], CG * EW);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -437,11 +487,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if constexpr (CG == 2) st_cluster_u32(mapa_shared(smem_u32(const_cast<int*>(abort_flag)), cta ^ 1u), 1u);
     };
 
-    // Registers: 168 a thread at launch; the first warpgroup gives up 112 of
-    // them, the two of the epilogue take 56 each (56 + 2 * 224 = 3 * 168).
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
         if (lane == 0) {
             const uint32_t full_leader = CG == 2 ? mapa_shared(smem_u32(full), 0u) : 0u;
             const uint32_t b_bytes = BMN ? (bn_cta > 64 ? 16384u : 8192u) : bn_cta * 128u;
@@ -515,7 +563,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------ UMMA issuer
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
         if (leader && lane == 0) {
             const uint32_t fmt = p.in_type == kBF16 ? 1u : 0u;
             const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (AMN ? 1u << 15 : 0u) |
@@ -574,22 +622,25 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------ epilogue
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pk_epi_regs(EW)));
         const int e = warp - 4;
         const uint32_t quarter = warp & 3;
-        const uint32_t half = e >> 2;
-        constexpr int kMaxChunks = 2 * CG;  // 32-column chunks per warp: 0, 2, .. or 1, 3, ..
-        const int chunks = static_cast<int>((bn_tile / 32 + 1 - half) / 2);
-        uint8_t* box = boxes + e * 2 * kPkBox;
+        const uint32_t group = e >> 2;
+        // 32-column chunks of this warp: number group, group + kGroups, ...
+        constexpr int kMaxChunks = 4 * CG / kGroups;
+        constexpr uint32_t kStep = 32 * kGroups;  // columns from one to the next
+        const int chunks = static_cast<int>((bn_tile / 32 + kGroups - 1 - group) / kGroups);
+        constexpr int kBox = kPkBoxes / EW / 2;
+        uint8_t* box = boxes + e * 2 * kBox;
         uint32_t nbox = 0;  // boxes sent: picks the buffer
         const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(tempty), 0u) : 0u;
-        const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + half * 32;
+        const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + group * 32;
         uint32_t acc = 0;
         bool ok = true;
 
         // The buffer of the next box, once the store that read it is done.
         auto next_box = [&]() -> uint8_t* {
-            uint8_t* b = box + (nbox & 1u) * kPkBox;
+            uint8_t* b = box + (nbox & 1u) * kBox;
             ++nbox;
             if (lane == 0) bulk_wait_read<1>();
             __syncwarp();
@@ -641,7 +692,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             if (lane == 0) bulk_commit();  // an empty group: the buffers keep taking turns
         };
         auto issue = [&](uint32_t buf, int i, float* v) {
-            tmem_ld_32cols(lane_base + buf * kBufCols + i * 64, reinterpret_cast<int32_t*>(v));
+            tmem_ld_32cols(lane_base + buf * kBufCols + i * kStep, reinterpret_cast<int32_t*>(v));
         };
         auto arrived = [&](float* v) { tmem_ld_wait_n<32>(reinterpret_cast<int32_t*>(v)); };
         auto release = [&](uint32_t buf) {
@@ -661,58 +712,65 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             tc_fence_after();
             return true;
         };
-        // Calls f(v, chunk) for this warp's chunks of the next tile, whose sums
-        // are in v. The tensor cores add into TMEM by truncation, which over a
-        // long K pulls every sum towards zero by parts in 10^5: K is summed
-        // there in pieces, and the pieces are added in registers, rounded to
-        // nearest.
-        auto for_tile = [&](uint32_t pieces, auto&& f) -> bool {
-            uint32_t buf;
-            if constexpr (!LONG) {
+        // The tensor cores add into TMEM by truncation, which over a long K
+        // pulls every sum towards zero by parts in 10^5: K is summed there in
+        // pieces, and the pieces are added in registers, rounded to nearest.
+        // This warp's chunks of the next tile, summed over its pieces.
+        auto sum_pieces = [&](uint32_t pieces, float* sums) -> bool {
+#pragma unroll
+            for (int j = 0; j < 32 * kMaxChunks; ++j) sums[j] = 0.0f;
+            for (uint32_t q = 0; q < pieces; ++q) {
+                uint32_t buf;
                 if (!wait_acc(buf)) return false;
-                float va[32], vb[32];
-                issue(buf, 0, va);
+                // Two chunks in flight at a time; the buffer goes back as soon
+                // as the last ones are in registers.
+#pragma unroll
+                for (int i = 0; i < kMaxChunks; i += 2) {
+                    float v[64];
+                    if (i < chunks) issue(buf, i, v);
+                    if (i + 1 < chunks) issue(buf, i + 1, v + 32);
+                    arrived(v);
+                    tie32(reinterpret_cast<int32_t*>(v + 32));
+                    if (i + 2 >= kMaxChunks) release(buf);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (i + h >= chunks) break;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float* s2 = sums + 32 * (i + h) + j;
+                            const float2 r = unpair_f32(add2(pair_f32(s2[0], s2[1]), pair_f32(v[32 * h + j], v[32 * h + j + 1])));
+                            s2[0] = r.x;
+                            s2[1] = r.y;
+                        }
+                    }
+                }
+            }
+            return true;
+        };
+        // Calls f(v, chunk) for this warp's chunks of the next tile. One call
+        // in the code: two copies of a long epilogue do not fit the
+        // instruction cache.
+        auto for_tile = [&](uint32_t pieces, auto&& f) -> bool {
+            if constexpr (!LONG) {
+                uint32_t buf;
+                if (!wait_acc(buf)) return false;
+                float next[32];
+                issue(buf, 0, next);
 #pragma unroll 1
-                for (int i = 0; i < chunks; i += 2) {
-                    arrived(va);
+                for (int i = 0; i < chunks; ++i) {
+                    float v[32];
+                    arrived(next);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = next[j];
                     if (i + 1 < chunks)
-                        issue(buf, i + 1, vb);
+                        issue(buf, i + 1, next);
                     else
                         release(buf);
-                    f(va, i);
-                    if (i + 1 < chunks) {
-                        arrived(vb);
-                        if (i + 2 < chunks)
-                            issue(buf, i + 2, va);
-                        else
-                            release(buf);
-                        f(vb, i + 1);
-                    }
+                    f(v, i);
                 }
             } else {
                 float sums[32 * kMaxChunks];
-#pragma unroll
-                for (int j = 0; j < 32 * kMaxChunks; ++j) sums[j] = 0.0f;
-                for (uint32_t q = 0; q < pieces; ++q) {
-                    if (!wait_acc(buf)) return false;
-                    float va[32], vb[32];
-                    issue(buf, 0, va);
-#pragma unroll
-                    for (int i = 0; i < kMaxChunks; i += 2) {
-                        arrived(va);
-                        if (i + 1 < chunks) issue(buf, i + 1, vb);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sums[32 * i + j] += va[j];
-                        if (i + 1 < chunks) {
-                            arrived(vb);
-                            if (i + 2 < chunks) issue(buf, i + 2, va);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) sums[32 * i + 32 + j] += vb[j];
-                        }
-                        if (i + 2 >= chunks) break;
-                    }
-                    release(buf);
-                }
+                if (!sum_pieces(pieces, sums)) return false;
 #pragma unroll
                 for (int i = 0; i < kMaxChunks; ++i)
                     if (i < chunks) f(sums + 32 * i, i);
@@ -728,10 +786,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 
             if constexpr (EPI == kEpiStore) {
                 const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
-                const uint32_t col_base = t.n0 * bn_tile + half * 32;
+                const uint32_t col_base = t.n0 * bn_tile + group * 32;
                 const uint32_t out_row0 = row0 + t.split * p.split_rows;
                 ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
-                    const uint32_t col = col_base + i * 64;
+                    const uint32_t col = col_base + i * kStep;
                     if (row0 >= p.m || col >= p.n) return;  // nobody reads what lies there
                     if (alpha != 1.0f) {
 #pragma unroll
@@ -819,44 +877,83 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 });
             } else if constexpr (EPI == kEpiSoftmax) {
                 // Running maximum (of the scaled logits, base 2) and sum of
-                // 2^(logit - maximum) of this row over its half of the columns,
+                // 2^(logit - maximum) of this row over this warp's columns,
                 // the label's column left out.
                 float top = -INFINITY, sum = 0.0f;
                 const int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
-                for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
-                    const uint32_t col_base = tn * bn_tile + half * 32;
-                    ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
-                        const uint32_t col = col_base + i * 64;
-                        const int32_t at = label - static_cast<int32_t>(col);
-                        if (at >= 0 && at < 32) {
-                            float z = 0.0f;
+                const uint64_t scale = pair_f32(p.scale2, p.scale2);
+                // Two chunks of a tile, from column col and col + kStep on. The
+                // special-function units set the pace (a polynomial on the FMA
+                // units for three eighths of the exponentials was slower, 707 us
+                // instead of 621: the issue slots are needed too), so the rest
+                // is two values an instruction.
+                auto soft = [&](float* v, uint32_t col) {
+                    const int32_t at = label - static_cast<int32_t>(col);
+                    constexpr int kNext = static_cast<int>(kStep);
+                    if ((at >= 0 && at < 32) || (at >= kNext && at < kNext + 32)) {
+                        const int32_t place = at < 32 ? at : at - kNext + 32;
+                        float z = 0.0f;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                z = j == at ? v[j] : z;
-                                v[j] = j == at ? -INFINITY : v[j];  // its term is added by the join
-                            }
-                            p.label_dot[row] = z;
+                        for (int j = 0; j < 64; ++j) {
+                            z = j == place ? v[j] : z;
+                            v[j] = j == place ? -INFINITY : v[j];  // its term is added by the join
                         }
-                        if (col + 32 > p.n) {  // past the last column: no weight
+                        p.label_dot[row] = z;
+                    }
+                    if (col + kStep + 32 > p.n) {  // past the last column: no weight
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (col + j >= p.n) v[j] = -INFINITY;
-                        }
-                        float big[4] = {v[0], v[1], v[2], v[3]};
+                        for (int j = 0; j < 64; ++j)
+                            if (col + (j < 32 ? j : kStep - 32 + j) >= p.n) v[j] = -INFINITY;
+                    }
+                    float big[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                        for (int j = 4; j < 32; ++j) big[j & 3] = fmaxf(big[j & 3], v[j]);
-                        const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-                        const float now = fmaxf(top, most * p.scale2);
-                        // A row whose logits so far are all -inf has no sum yet.
-                        const float base = now == -INFINITY ? 0.0f : now;
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int j = 4; j < 60; j += 8)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(v[j], p.scale2, -base));
-                        sum = sum * exp2_approx(top - base) + ((part[0] + part[1]) + (part[2] + part[3]));
-                        top = now;
-                    });
+                        for (int h = 0; h < 4; ++h) big[h] = max3(big[h], v[j + 2 * h], v[j + 2 * h + 1]);
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) big[h] = fmaxf(big[h], v[60 + h]);
+                    const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+                    const float now = fmaxf(top, most * p.scale2);
+                    // A row whose logits so far are all -inf has no sum yet.
+                    const float base = now == -INFINITY ? 0.0f : now;
+                    const uint64_t minus = pair_f32(-base, -base);
+                    uint64_t part[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2) {
+                        const uint64_t x = fma2(pair_f32(v[j], v[j + 1]), scale, minus);
+                        const float2 f = unpair_f32(x);
+                        const uint64_t e = pair_f32(exp2_approx(f.x), exp2_approx(f.y));
+                        part[(j >> 1) & 3] = add2(part[(j >> 1) & 3], e);
+                    }
+                    const float2 s2 = unpair_f32(add2(add2(part[0], part[1]), add2(part[2], part[3])));
+                    sum = fmaf(sum, exp2_approx(top - base), s2.x + s2.y);
+                    top = now;
+                };
+                // Tiles here are whole (128 * CG columns): batches of two chunks a warp.
+                if constexpr (LONG) {
+                    for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
+                        float sums[32 * kMaxChunks];
+                        ok = sum_pieces(t.p1 - t.p0, sums);
+                        if (!ok) break;
+#pragma unroll
+                        for (int i = 0; i < kMaxChunks; i += 2) soft(sums + 32 * i, tn * bn_tile + group * 32 + i * kStep);
+                    }
+                } else {
+                    static_assert(LONG || kMaxChunks == 2, "one batch");
+                    for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
+                        uint32_t buf;
+                        ok = wait_acc(buf);
+                        if (!ok) break;
+                        float v[64];
+                        issue(buf, 0, v);
+                        issue(buf, 1, v + 32);
+                        arrived(v);
+                        tie32(reinterpret_cast<int32_t*>(v + 32));
+                        release(buf);
+                        soft(v, tn * bn_tile + group * 32);
+                    }
                 }
-                if (ok && live) p.part[uint64_t(2 * t.segment + half) * p.m + row] = make_float2(top, sum);
+                if (ok && live) p.part[uint64_t(kGroups * t.segment + group) * p.m + row] = make_float2(top, sum);
             } else {
                 const float lse2 = live ? p.lse2[row] : 0.0f;
                 const float cmax_inv = *p.alpha_dev > 0.0f ? 1.0f / *p.alpha_dev : 0.0f;
@@ -864,14 +961,21 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 // Column of the row's class here; negative where it has none or an earlier piece holds it.
                 int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;
                 if (label >= 0) label -= static_cast<int32_t>(p.class0);
-                const uint32_t col_base = t.n0 * bn_tile + half * 32;
+                const uint32_t col_base = t.n0 * bn_tile + group * 32;
+                const uint64_t scale = pair_f32(p.scale2, p.scale2), minus = pair_f32(-lse2, -lse2);
+                const uint64_t weight = pair_f32(coef, coef);
                 // Planes are read in whole K blocks of 64 columns.
                 const uint32_t width = p.grad_planes == 1 ? p.n : (p.n + 63) / 64 * 64;
                 ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
-                    const uint32_t col = col_base + i * 64;
+                    const uint32_t col = col_base + i * kStep;
                     if (row0 >= p.m || col >= width) return;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = coef * exp2_approx(fmaf(v[j], p.scale2, -lse2));
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 x = unpair_f32(fma2(pair_f32(v[j], v[j + 1]), scale, minus));
+                        const float2 g = unpair_f32(mul2(pair_f32(exp2_approx(x.x), exp2_approx(x.y)), weight));
+                        v[j] = g.x;
+                        v[j + 1] = g.y;
+                    }
                     const int32_t at = label - static_cast<int32_t>(col);
                     if (at >= 0 && at < 32) {
                         float g = 0.0f;
@@ -916,7 +1020,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (lane == 0) bulk_wait_all();
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
     }
 
     tc_fence_before();
