@@ -227,12 +227,12 @@ struct Shape {
 
 // K blocks of 64 summed by the tensor cores alone, whose additions truncate:
 // 1024 of K where 16 bits come of it, 256 (bf16) or 128 (fp16, whose products
-// are longer, and fp32) where the result stays fp32. Loss of 2048 rows of
+// are longer) where the result stays fp32, 64 for six plane products. Loss of 2048 rows of
 // width 960 against 30,000, relative error against 64 bits: bf16 1.3e-6 at 128,
 // 2.4e-6 at 256 (and 1046 us instead of 1257 for 8192 rows against 100,000);
 // fp16 2.3e-6 and 5.5e-6; plain fp32 3.6e-6 and 4.4e-6. A 16-bit result has
 // 2e-4 or more of its own.
-uint32_t piece_blocks(const Shape& s) { return !s.precise ? 16u : s.bf16 ? 4u : 2u; }
+uint32_t piece_blocks(const Shape& s) { return !s.precise ? 16u : s.bf16 ? 4u : s.combos == 1 ? 2u : 1u; }
 
 struct Plan {
     int cg;
@@ -261,25 +261,29 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
 // item its K blocks and a fixed part (first loads, last stores, schedule); a
 // launch of pairs takes some 3 us longer to get going than one of single CTAs.
 // A K block costs the tensor cores 2 cycles per column of the tile (a pair
-// does 256 rows at once, a single CTA 128), and its 16 KiB of A and 128 bytes
-// per row of B about 60 bytes per cycle from L2: the single tiles and narrow
-// ones are bound by that. A split product is written, read and joined in fp32
-// by another kernel.
+// does 256 rows at once, a single CTA 128) and plane product, and its 16 KiB of
+// A and 128 bytes per row of B and plane about 60 bytes per cycle from L2: the
+// single tiles and narrow ones are bound by that. A split product is written
+// and read in fp32 once more, some 3400 bytes a cycle, and may need another
+// kernel to join it.
 double plan_cycles(const Plan& q, const Shape& s)
 {
     const uint64_t units = sm_count() / q.cg;
     const uint64_t items = uint64_t(q.tiles_m) * q.tiles_n * q.splits;
     const double rounds = static_cast<double>(ceil_div(items, units));
-    const double block = std::max(2.0 * q.tile_n, (16384.0 + 128.0 * q.tile_n / q.cg) / 60.0);
-    const double blocks = static_cast<double>(ceil_div(q.pieces(), q.splits)) * q.piece * s.combos;
+    const double planes = s.combos == 1 ? 1.0 : 3.0;
+    const double block =
+        std::max(2.0 * s.combos * q.tile_n, planes * (16384.0 + 128.0 * q.tile_n / q.cg) / 60.0);
+    const double blocks = static_cast<double>(ceil_div(q.pieces(), q.splits)) * q.piece;
     double cycles = rounds * (blocks * block + 1500.0) + (q.cg == 2 ? 6000.0 : 0.0);
-    if (q.splits > 1) cycles += 6000.0 + static_cast<double>(s.m) * s.n * q.splits * 8.0 / 3000.0;
+    if (q.splits > 1) cycles += 6000.0 + static_cast<double>(s.m) * s.n * q.splits * 8.0 / 3400.0;
     return cycles;
 }
 
 // The cheapest of pairs (256 rows) and single CTAs (128 rows) with tiles from
-// 64 columns up, the K loop whole or cut into 2, 4, 8, ... splits of at least
-// four K blocks, up to as many as fill the units.
+// 64 columns up, the K loop whole or cut into 2, 3, 4, 6, 8, ... splits of at
+// least four K blocks: where the tiles leave units idle, up to as many as fill
+// them; where they do not, up to eight, to even out the last round.
 Plan plan_product(const Shape& s)
 {
     Plan best;
@@ -290,8 +294,10 @@ Plan plan_product(const Shape& s)
             const uint32_t whole = q.piece;
             const uint64_t tiles = uint64_t(q.tiles_m) * q.tiles_n;
             const uint64_t units = sm_count() / cg;
-            const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(units / tiles, q.kblocks / ceil_div(4, s.combos)));
-            for (uint64_t want = 1;; want = std::min(2 * want, most)) {
+            const uint64_t longest = q.kblocks / ceil_div(4, s.combos);
+            const uint64_t most = std::max<uint64_t>(
+                1, std::min<uint64_t>(tiles < units ? units / tiles : tiles < 8 * units ? 8 : 1, longest));
+            for (uint64_t want = 1;;) {
                 q.piece = static_cast<uint32_t>(std::min<uint64_t>(whole, ceil_div(q.kblocks, want)));
                 q.splits = static_cast<uint32_t>(std::min<uint64_t>(want, q.pieces()));
                 const double c = plan_cycles(q, s);
@@ -300,6 +306,7 @@ Plan plan_product(const Shape& s)
                     best = q;
                 }
                 if (want == most) break;
+                want = std::min(want < 4 ? want + 1 : want % 3 ? want + want / 2 : want + want / 3, most);
             }
         }
     }
@@ -416,7 +423,7 @@ ProductParams base_params(const Shape& s, const Plan& q, const Operand& a, const
     p.kblocks = q.kblocks;
     p.piece = q.piece;
     p.pieces = q.pieces();
-    p.combos = s.combos;
+    p.planes = s.combos == 1 ? 1 : 3;
     p.plane_a = a.plane;
     p.plane_b = b.plane;
     p.in_type = operand_type(dtype);

@@ -244,37 +244,52 @@ struct SlopeParams {
     int vec;              // rows of dy and pre allow 16-byte loads
 };
 
-__device__ __forceinline__ void load8(const void* p, uint64_t at, int type, uint32_t left, bool vec, float* v)
-{
-    if (vec && left >= 8) {
-        if (type == kF32) {
-            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-            const float4 a = q[0], b = q[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// 8 consecutive values as they lie; those past `left` are zeros.
+template <int TYPE>
+struct Octet {
+    uint32_t w[TYPE == kF32 ? 8 : 4];
+
+    __device__ __forceinline__ void load(const void* p, uint64_t at, uint32_t left, bool whole)
+    {
+        constexpr int kWords = TYPE == kF32 ? 8 : 4;
+        if (whole) {
+            const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (kWords / 2));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = unpack2(w[j], type);
-                v[2 * j] = f.x;
-                v[2 * j + 1] = f.y;
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 v = __ldcs(q + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
-        }
-    } else {
+        } else if constexpr (TYPE == kF32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < static_cast<int>(left) ? load_elem(p, at + j, type) : 0.0f;
+            for (int j = 0; j < 8; ++j) w[j] = j < static_cast<int>(left) ? static_cast<const uint32_t*>(p)[at + j] : 0u;
+        } else {
+            const uint16_t* h = static_cast<const uint16_t*>(p) + at;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = (2 * j < static_cast<int>(left) ? h[2 * j] : 0u) |
+                       (2 * j + 1 < static_cast<int>(left) ? static_cast<uint32_t>(h[2 * j + 1]) << 16 : 0u);
+        }
     }
-}
+    // Values 2 j and 2 j + 1.
+    __device__ __forceinline__ uint64_t pair(int j) const
+    {
+        if constexpr (TYPE == kF32) return pair_f32(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+        const float2 f = unpack2(w[j], TYPE);
+        return pair_f32(f.x, f.y);
+    }
+};
 
 // dz = dy act'(pre), rounded to the operands' type, and its column sums (of
-// the unrounded values). A block takes 256 columns (8 per lane) and a range of
-// rows; its 8 warps take every eighth row, two at a time so that four 16-byte
-// loads a thread are in flight, and add up their sums in order.
+// the unrounded values). Bound by HBM: dy and pre in, dz out. A block takes 256
+// columns (8 per lane) and a range of rows; its 8 warps take every eighth row,
+// the loads of the next rows on their way while the current ones are worked
+// on, and add up their sums in order.
 template <int ACT, int TYPE>
 __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopeParams p)
 {
+    constexpr int kRows = TYPE == kF32 ? 1 : 2;  // of a warp at a time
+    constexpr int kOut = TYPE == kF16 ? kF16 : kBF16;
+    constexpr int kPlanes = TYPE == kF32 ? 3 : 1;
     __shared__ float total[8][256];
     previous_done();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,38 +297,51 @@ __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopePar
     const uint64_t r0 = p.m * blockIdx.y / gridDim.y, r1 = p.m * (blockIdx.y + 1) / gridDim.y;
     const uint32_t left = c0 < p.n ? p.n - c0 : 0;
     const bool whole = p.vec && left >= 8;
-    float acc[8] = {};
-    for (uint64_t r = r0 + warp; r < r1; r += 16) {
-        float v[2][8] = {}, z[2][8] = {};
+    uint64_t acc[4] = {0, 0, 0, 0};
+    Octet<TYPE> dy[kRows], z[kRows];
+    const auto fetch = [&](uint64_t r) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (left && r + 8 * h < r1) {
-                load8(p.dy, (r + 8 * h) * p.lddy + c0, TYPE, left, whole, v[h]);
-                if constexpr (ACT != kActNone) load8(p.pre, (r + 8 * h) * p.ldp + c0, TYPE, left, whole, z[h]);
-            }
+        for (int h = 0; h < kRows; ++h) {
+            const bool there = left && r + 8 * h < r1;
+            const uint64_t row = there ? r + 8 * h : 0;
+            dy[h].load(p.dy, row * p.lddy + c0, there ? left : 0, there && whole);
+            if constexpr (ACT != kActNone) z[h].load(p.pre, row * p.ldp + c0, there ? left : 0, there && whole);
         }
+    };
+    fetch(r0 + warp);
+    for (uint64_t r = r0 + warp; r < r1; r += 8 * kRows) {
+        Octet<TYPE> d[kRows], u[kRows];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kRows; ++h) {
+            d[h] = dy[h];
+            u[h] = z[h];
+        }
+        fetch(r + 8 * kRows);
+#pragma unroll
+        for (int h = 0; h < kRows; ++h) {
             if (r + 8 * h >= r1) break;
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (ACT != kActNone) v[h][j] *= slope_f<ACT>(z[h][j]);
-                acc[j] += v[h][j];
+            for (int j = 0; j < 4; ++j) {
+                uint64_t g = d[h].pair(j);
+                if constexpr (ACT != kActNone) g = mul2(g, slope2<ACT>(u[h].pair(j)));
+                acc[j] = add2(acc[j], g);
+                const float2 f = unpair_f32(g);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
             }
             if (p.out && c0 < p.pitch) {
-                constexpr int kOut = TYPE == kF16 ? kF16 : kBF16;
-                constexpr int kPlanes = TYPE == kF32 ? 3 : 1;
                 uint16_t* dst = p.out + (r + 8 * h) * (uint64_t(p.pitch) * kPlanes) + c0;
 #pragma unroll
                 for (int plane = 0; plane < kPlanes; ++plane) {
                     uint32_t w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        w[j] = pack2(v[h][2 * j], v[h][2 * j + 1], kOut);
+                        w[j] = pack2(v[2 * j], v[2 * j + 1], kOut);
                         if (plane + 1 < kPlanes) {
                             const float2 f = unpack2(w[j], kOut);
-                            v[h][2 * j] -= f.x;
-                            v[h][2 * j + 1] -= f.y;
+                            v[2 * j] -= f.x;
+                            v[2 * j + 1] -= f.y;
                         }
                     }
                     *reinterpret_cast<uint4*>(dst + plane * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -323,7 +351,11 @@ __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopePar
     }
     if (p.sums) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) total[warp][lane * 8 + j] = acc[j];
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpair_f32(acc[j]);
+            total[warp][lane * 8 + 2 * j] = f.x;
+            total[warp][lane * 8 + 2 * j + 1] = f.y;
+        }
         __syncthreads();
         const uint32_t c = blockIdx.x * 256 + threadIdx.x;
         if (c < p.n) {

@@ -10,8 +10,9 @@
 // Operands are bf16 or fp16 with fp32 accumulation in TMEM. fp32 operands come
 // as three bf16 planes (x = h + m + l, each the rounding of what the ones
 // before left) and the product is the six plane products down to 2^-18 of the
-// leading one, summed smallest first into the same accumulator; the three that
-// are left out are below 2^-26 of it.
+// leading one, summed into the same accumulator; the three that are left out
+// are below 2^-26 of it. Each plane of a K block is staged once and read by all
+// the products that need it.
 //
 // Tile and roles. CG = 2: a CTA pair computes up to 256 x 256 with
 // tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and half the tile's
@@ -58,7 +59,7 @@ struct ProductParams {
     uint32_t kblocks;              // 64-wide K blocks of one plane
     uint32_t piece;                // K blocks (of every plane product) summed in TMEM before they leave it
     uint32_t pieces;               // ceil(kblocks / piece)
-    uint32_t combos;               // 1, or 6 plane products of split fp32 operands
+    uint32_t planes;               // 1, or 3 parts of split fp32 operands
     uint32_t plane_a, plane_b;     // columns from one plane to the next in the stored matrices
     int in_type;                   // kBF16 or kF16
     int* error;
@@ -236,59 +237,95 @@ __device__ __forceinline__ float rcp_approx(float x)
     return y;
 }
 
+__device__ __forceinline__ uint64_t both(float c) { return pair_f32(c, c); }
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x)
+{
+    const float2 f = unpair_f32(x);
+    return pair_f32(exp2_approx(f.x), exp2_approx(f.y));
+}
+__device__ __forceinline__ uint64_t rcp_pair(uint64_t x)
+{
+    const float2 f = unpair_f32(x);
+    return pair_f32(rcp_approx(f.x), rcp_approx(f.y));
+}
+
+// The activations and their slopes, two values at a time: the epilogues that
+// use them are bound by issue slots.
+
 // sigmoid(v) = 1 / (1 + e^-v); e^-v overflows to +inf for very negative v,
 // where the quotient is 0 as it should be.
-__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.0f + exp2_approx(-1.44269504f * v)); }
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t v)
+{
+    return rcp_pair(add2(exp2_pair(mul2(v, both(-1.44269504f))), both(1.0f)));
+}
 
 // The normal distribution function Phi(z) and *bell = e^(-z^2 / 2), by
 // Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2) with
 // t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7 for x = |z| / sqrt 2 >= 0.
-// No branch, and the gradient needs the same exponential.
-__device__ __forceinline__ float normal_cdf(float z, float* bell)
+// No branch, and the slope needs the same exponential. q is Phi(-|z|) =
+// erfc(x) / 2, and Phi(z) = 1/2 + (1/2 - q) with the sign of z.
+__device__ __forceinline__ uint64_t normal_cdf2(uint64_t z, uint64_t* bell)
 {
-    const float e = exp2_approx(-0.72134752f * z * z);
-    const float t = rcp_approx(fmaf(fabsf(z), 0.23164189f, 1.0f));
-    float q = fmaf(t, 0.530702715f, -0.726576014f);  // half the coefficients: Phi(-|z|) = erfc(x) / 2
-    q = fmaf(t, q, 0.710706871f);
-    q = fmaf(t, q, -0.142248368f);
-    q = fmaf(t, q, 0.127414796f);
-    q = q * t * e;
+    const uint64_t e = exp2_pair(mul2(mul2(z, z), both(-0.72134752f)));
+    const uint64_t t = rcp_pair(fma2(z & 0x7FFFFFFF7FFFFFFFull, both(0.23164189f), both(1.0f)));
+    uint64_t q = fma2(t, both(0.530702715f), both(-0.726576014f));  // half the coefficients
+    q = fma2(t, q, both(0.710706871f));
+    q = fma2(t, q, both(-0.142248368f));
+    q = fma2(t, q, both(0.127414796f));
+    q = mul2(mul2(q, t), e);
     *bell = e;
-    return z < 0.0f ? q : 1.0f - q;
+    const uint64_t r = fma2(q, both(-1.0f), both(0.5f));
+    return add2((r & 0x7FFFFFFF7FFFFFFFull) | (z & 0x8000000080000000ull), both(0.5f));
+}
+
+template <int ACT>
+__device__ __forceinline__ uint64_t act2(uint64_t z)
+{
+    if constexpr (ACT == kActRelu) {
+        const float2 f = unpair_f32(z);
+        return pair_f32(f.x < 0.0f ? 0.0f : f.x, f.y < 0.0f ? 0.0f : f.y);  // NaN stays NaN
+    }
+    if constexpr (ACT == kActGelu) {
+        uint64_t bell;
+        return mul2(z, normal_cdf2(z, &bell));
+    }
+    // 0.5 (1 + tanh u) = sigmoid(2 u), 2 u = z (c + 0.044715 c z^2), c = 2 sqrt(2/pi).
+    if constexpr (ACT == kActGeluTanh)
+        return mul2(z, sigmoid2(mul2(z, fma2(mul2(z, z), both(0.0713548163f), both(1.59576912f)))));
+    if constexpr (ACT == kActSilu) return mul2(z, sigmoid2(z));
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ uint64_t slope2(uint64_t z)
+{
+    if constexpr (ACT == kActRelu) {
+        const float2 f = unpair_f32(z);
+        return pair_f32(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f);
+    }
+    if constexpr (ACT == kActGelu) {
+        uint64_t bell;
+        const uint64_t phi = normal_cdf2(z, &bell);
+        return fma2(mul2(z, both(0.39894228f)), bell, phi);
+    }
+    if constexpr (ACT == kActGeluTanh) {
+        const uint64_t zz = mul2(z, z);
+        const uint64_t s = sigmoid2(mul2(z, fma2(zz, both(0.0713548163f), both(1.59576912f))));
+        const uint64_t du = fma2(zz, both(0.214064449f), both(1.59576912f));
+        // s + z s (1 - s) du
+        return fma2(mul2(mul2(z, s), fma2(s, both(-1.0f), both(1.0f))), du, s);
+    }
+    if constexpr (ACT == kActSilu) {
+        const uint64_t s = sigmoid2(z);
+        return mul2(s, fma2(z, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
+    }
+    return both(1.0f);
 }
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float z)
 {
-    if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    if constexpr (ACT == kActGelu) {
-        float bell;
-        return z * normal_cdf(z, &bell);
-    }
-    // 0.5 (1 + tanh u) = sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3).
-    if constexpr (ACT == kActGeluTanh) return z * sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
-    if constexpr (ACT == kActSilu) return z * sigmoid_f(z);
-    return z;
-}
-
-template <int ACT>
-__device__ __forceinline__ float slope_f(float z)
-{
-    if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
-    if constexpr (ACT == kActGelu) {
-        float bell;
-        const float phi = normal_cdf(z, &bell);
-        return fmaf(0.39894228f * z, bell, phi);
-    }
-    if constexpr (ACT == kActGeluTanh) {
-        const float s = sigmoid_f(1.59576912f * (z + 0.044715f * z * z * z));
-        return s + z * s * (1.0f - s) * 1.59576912f * (1.0f + 0.134145f * z * z);
-    }
-    if constexpr (ACT == kActSilu) {
-        const float s = sigmoid_f(z);
-        return s * (1.0f + z * (1.0f - s));
-    }
-    return 1.0f;
+    return unpair_f32(act2<ACT>(both(z))).x;
 }
 
 // One value of the linear epilogue (shared with the join of split products).
@@ -345,18 +382,11 @@ template <int ACT>
 __device__ __forceinline__ void act_all(float* v)
 {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_f<ACT>(v[i]);
-}
-
-// The A / B plane of plane product c, smallest products first:
-// l h, h l, m m, m h, h m, h h.
-__device__ __forceinline__ uint32_t combo_a(uint32_t c, uint32_t combos)
-{
-    return combos == 1 ? 0u : (0x001102u >> (4 * c)) & 3u;  // 2,0,1,1,0,0
-}
-__device__ __forceinline__ uint32_t combo_b(uint32_t c, uint32_t combos)
-{
-    return combos == 1 ? 0u : (0x010120u >> (4 * c)) & 3u;  // 0,2,1,0,1,0
+    for (int i = 0; i < 32; i += 2) {
+        const float2 r = unpair_f32(act2<ACT>(pair_f32(v[i], v[i + 1])));
+        v[i] = r.x;
+        v[i + 1] = r.y;
+    }
 }
 
 // Class of a row, -1 where it has none.
@@ -406,11 +436,15 @@ __device__ __forceinline__ Item decode_item(const ProductParams& p, uint32_t i)
 }
 
 // ---------------------------------------------------------------- kernel
-// Epilogue warps: 16 where a pair's tile goes through exponentials (with two
-// warps per scheduler the special-function units idle through every latency:
-// 2048 x 128 against a million rows took 621 us with 8), 8 elsewhere: long sums
-// and stores need the registers.
-__host__ __device__ constexpr int pk_epi_warps(int cg, int epi, bool longk) { return cg == 2 && epi != kEpiStore && !longk ? 16 : 8; }
+// Epilogue warps: 16, or 8 where sums over long K need the registers and for
+// the softmax of single CTAs, whose warps take two chunks at once. With 8, two
+// warps per scheduler leave every latency of an epilogue exposed: 2048 x 128
+// against a million rows took 621 us instead of 572, a gelu layer of 100,000 x
+// 784 -> 1024 249 us instead of 189.
+__host__ __device__ constexpr int pk_epi_warps(int cg, int epi, bool longk)
+{
+    return longk || (cg == 1 && epi == kEpiSoftmax) ? 8 : 16;
+}
 __host__ __device__ constexpr int pk_threads(int cg, int epi, bool longk) { return 128 + 32 * pk_epi_warps(cg, epi, longk); }
 // Registers a thread: what the launch gives, and the split after setmaxnreg
 // between the first warpgroup and those of the epilogue. The split never sums
@@ -501,20 +535,16 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                 const int32_t am = static_cast<int32_t>(t.tm * (128 * CG) + cta * 128);
                 for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
                     const int32_t bn = static_cast<int32_t>(tn * bn_tile + cta * bn_cta);
-                    uint32_t piece = t.p0, c = 0, kb = t.p0 * p.piece;
-                    while (piece < t.p1) {
-                        const uint32_t kb1 = min((piece + 1) * p.piece, p.kblocks);
+                    const uint32_t kb1 = min(t.p1 * p.piece, p.kblocks);
+                    uint32_t kb = t.p0 * p.piece, plane = p.planes;
+                    while (kb < kb1) {
                         const int32_t k = static_cast<int32_t>(kb * 64);
-                        const int32_t pa = static_cast<int32_t>(combo_a(c, p.combos) * p.plane_a);
-                        const int32_t pb = static_cast<int32_t>(combo_b(c, p.combos) * p.plane_b);
-                        // K blocks of a piece, then the next plane product, then the next piece.
-                        if (++kb == kb1) {
-                            kb = piece * p.piece;
-                            if (++c == p.combos) {
-                                c = 0;
-                                kb = kb1;
-                                ++piece;
-                            }
+                        --plane;  // the smallest plane of a K block first
+                        const int32_t pa = static_cast<int32_t>(plane * p.plane_a);
+                        const int32_t pb = static_cast<int32_t>(plane * p.plane_b);
+                        if (plane == 0) {
+                            plane = p.planes;
+                            ++kb;
                         }
                         ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_limit);
                         if (!ok) break;
@@ -581,33 +611,73 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                 const uint32_t pieces = (t.n1 - t.n0) * (t.p1 - t.p0);
                 for (uint32_t q = 0; ok && q < pieces; ++q, ++acc) {
                     const uint32_t piece = t.p0 + q % (t.p1 - t.p0);
-                    const uint32_t blocks = (min((piece + 1) * p.piece, p.kblocks) - piece * p.piece) * p.combos;
+                    const uint32_t blocks = min((piece + 1) * p.piece, p.kblocks) - piece * p.piece;
                     const uint32_t buf = acc & 1u;
                     ok = mbar_wait_sleep(&tempty[buf], ((acc >> 1) & 1u) ^ 1u, abort_flag, p.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem_base + buf * kBufCols;
-                    for (uint32_t kk = 0; kk < blocks; ++kk) {
-                        ok = mbar_wait_sleep(&full[stage], phase, abort_flag, p.wait_limit);
-                        if (!ok) break;
+                    auto stage_ready = [&]() {
+                        const bool r = mbar_wait_sleep(&full[stage], phase, abort_flag, p.wait_limit);
                         tc_fence_after();
-                        const uint64_t ad = a0 + stage * (kPkStageBytes >> 4);
-                        const uint64_t bd = b0 + stage * (kPkStageBytes >> 4);
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) {
-                            const uint32_t more = (kk > 0 || ks > 0) ? 1u : 0u;
-                            if constexpr (CG == 2)
-                                umma_f16_pair(d, ad + ks * ka, bd + ks * kb, idesc, more);
-                            else
-                                umma_f16(d, ad + ks * ka, bd + ks * kb, idesc, more);
-                        }
-                        if constexpr (CG == 2)
-                            umma_commit_pair(&empty[stage]);
-                        else
-                            umma_commit(&empty[stage]);
+                        return r;
+                    };
+                    auto next_stage = [&]() {
                         if (++stage == kPkStages) {
                             stage = 0;
                             phase ^= 1;
+                        }
+                    };
+                    // One K block of stage sa's A against stage sb's B.
+                    auto multiply = [&](uint32_t sa, uint32_t sb, bool more) {
+                        const uint64_t ad = a0 + sa * (kPkStageBytes >> 4);
+                        const uint64_t bd = b0 + sb * (kPkStageBytes >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t add = more || ks > 0 ? 1u : 0u;
+                            if constexpr (CG == 2)
+                                umma_f16_pair(d, ad + ks * ka, bd + ks * kb, idesc, add);
+                            else
+                                umma_f16(d, ad + ks * ka, bd + ks * kb, idesc, add);
+                        }
+                    };
+                    auto stage_done = [&](uint32_t s) {
+                        if constexpr (CG == 2)
+                            umma_commit_pair(&empty[s]);
+                        else
+                            umma_commit(&empty[s]);
+                    };
+                    if (p.planes == 1) {
+                        for (uint32_t kk = 0; kk < blocks; ++kk) {
+                            ok = stage_ready();
+                            if (!ok) break;
+                            multiply(stage, stage, kk > 0);
+                            stage_done(stage);
+                            next_stage();
+                        }
+                    } else {
+                        // Planes l, m, h of a K block, the small products first:
+                        // each addition costs a truncation of what is there.
+                        // A piece is one K block here, so the accumulator holds
+                        // only small sums until the last product.
+                        for (uint32_t kk = 0; kk < blocks; ++kk) {
+                            uint32_t at[3];
+#pragma unroll
+                            for (int plane = 2; plane >= 0; --plane) {
+                                if (ok) ok = stage_ready();
+                                at[plane] = stage;
+                                next_stage();
+                            }
+                            if (!ok) break;
+                            multiply(at[0], at[2], kk > 0);
+                            multiply(at[2], at[0], true);
+                            stage_done(at[2]);
+                            multiply(at[1], at[1], true);
+                            multiply(at[1], at[0], true);
+                            multiply(at[0], at[1], true);
+                            stage_done(at[1]);
+                            multiply(at[0], at[0], true);
+                            stage_done(at[0]);
                         }
                     }
                     if (!ok) break;
@@ -638,11 +708,18 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         uint32_t acc = 0;
         bool ok = true;
 
-        // The buffer of the next box, once the store that read it is done.
-        auto next_box = [&]() -> uint8_t* {
-            uint8_t* b = box + (nbox & 1u) * kBox;
+        // The buffer of the next box, once the store that read it is done. Two
+        // take turns; an fp32 box of 4 KiB may need the room of both.
+        auto next_box = [&](bool f32 = false) -> uint8_t* {
+            const bool one = kBox < 4096 && f32;
+            uint8_t* b = box + (one ? 0u : (nbox & 1u) * kBox);
             ++nbox;
-            if (lane == 0) bulk_wait_read<1>();
+            if (lane == 0) {
+                if (one)
+                    bulk_wait_read<0>();
+                else
+                    bulk_wait_read<1>();
+            }
             __syncwarp();
             return b;
         };
@@ -747,25 +824,18 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
             }
             return true;
         };
-        // Calls f(v, chunk) for this warp's chunks of the next tile. One call
-        // in the code: two copies of a long epilogue do not fit the
-        // instruction cache.
+        // Calls f(v, chunk) for this warp's chunks of the next tile.
         auto for_tile = [&](uint32_t pieces, auto&& f) -> bool {
             if constexpr (!LONG) {
                 uint32_t buf;
                 if (!wait_acc(buf)) return false;
-                float next[32];
-                issue(buf, 0, next);
+                if (chunks == 0) release(buf);
 #pragma unroll 1
                 for (int i = 0; i < chunks; ++i) {
                     float v[32];
-                    arrived(next);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = next[j];
-                    if (i + 1 < chunks)
-                        issue(buf, i + 1, next);
-                    else
-                        release(buf);
+                    issue(buf, i, v);
+                    arrived(v);
+                    if (i + 1 == chunks) release(buf);
                     f(v, i);
                 }
             } else {
@@ -819,7 +889,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                     }
                     if (p.pre) {
                         // The value before the activation, rounded to the inputs' type.
-                        uint8_t* b = next_box();
+                        uint8_t* b = next_box(p.aux_type == kF32);
                         if (p.aux_type == kF32) {
                             put_f32(b, v);
                         } else {
@@ -862,7 +932,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                                 if (col + j < p.n) v[j] += load_elem(p.residual, at + j, p.aux_type);
                         }
                     }
-                    uint8_t* b = next_box();
+                    uint8_t* b = next_box(p.out_type == kF32 || p.aux_type == kF32);
                     if (p.out_type == kF32) {
                         put_f32(b, v);
                     } else {
