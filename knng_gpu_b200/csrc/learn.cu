@@ -261,19 +261,21 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
 // item its K blocks and a fixed part (first loads, last stores, schedule); a
 // launch of pairs takes some 3 us longer to get going than one of single CTAs.
 // A K block costs the tensor cores 2 cycles per column of the tile (a pair
-// does 256 rows at once, a single CTA 128) and plane product, and its 16 KiB of
-// A and 128 bytes per row of B and plane about 60 bytes per cycle from L2: the
-// single tiles and narrow ones are bound by that. A split product is written
-// and read in fp32 once more, some 3400 bytes a cycle, and may need another
-// kernel to join it.
+// does 256 rows at once, a single CTA 128) and plane product. Its 16 KiB of A
+// and 128 bytes per row of B, for each plane, come from L2 at about 60 bytes a
+// cycle and go into shared memory, from where every plane product reads them
+// once, at 128 bytes a cycle: single tiles and narrow ones are bound by that. A
+// split product is written and read in fp32 once more, some 3400 bytes a
+// cycle, and may need another kernel to join it.
 double plan_cycles(const Plan& q, const Shape& s)
 {
     const uint64_t units = sm_count() / q.cg;
     const uint64_t items = uint64_t(q.tiles_m) * q.tiles_n * q.splits;
     const double rounds = static_cast<double>(ceil_div(items, units));
     const double planes = s.combos == 1 ? 1.0 : 3.0;
+    const double bytes = 16384.0 + 128.0 * q.tile_n / q.cg;
     const double block =
-        std::max(2.0 * s.combos * q.tile_n, planes * (16384.0 + 128.0 * q.tile_n / q.cg) / 60.0);
+        std::max({2.0 * s.combos * q.tile_n, (planes + s.combos) * bytes / 128.0, planes * bytes / 60.0});
     const double blocks = static_cast<double>(ceil_div(q.pieces(), q.splits)) * q.piece;
     double cycles = rounds * (blocks * block + 1500.0) + (q.cg == 2 ? 6000.0 : 0.0);
     if (q.splits > 1) cycles += 6000.0 + static_cast<double>(s.m) * s.n * q.splits * 8.0 / 3400.0;
@@ -284,7 +286,7 @@ double plan_cycles(const Plan& q, const Shape& s)
 // 64 columns up, the K loop whole or cut into 2, 3, 4, 6, 8, ... splits of at
 // least four K blocks: where the tiles leave units idle, up to as many as fill
 // them; where they do not, up to eight, to even out the last round.
-Plan plan_product(const Shape& s)
+Plan search_plan(const Shape& s)
 {
     Plan best;
     double least = 0.0;
@@ -311,6 +313,24 @@ Plan plan_product(const Shape& s)
         }
     }
     return best;
+}
+
+// The search takes some microseconds of host time: a thread keeps the plans of
+// the shapes it met last.
+Plan plan_product(const Shape& s)
+{
+    struct Entry {
+        Shape s;
+        Plan q;
+    };
+    thread_local Entry kept[64] = {};
+    const uint64_t key = (s.m * 0x9E3779B97F4A7C15ull + s.n) * 0xC2B2AE3D27D4EB4Full + s.k * 0x165667B19E3779F9ull +
+                         s.combos * 4 + s.precise * 2 + s.bf16;
+    Entry& e = kept[(key ^ (key >> 29)) & 63];
+    if (e.s.m != s.m || e.s.n != s.n || e.s.k != s.k || e.s.combos != s.combos || e.s.precise != s.precise ||
+        e.s.bf16 != s.bf16)
+        e = Entry{s, search_plan(s)};
+    return e.q;
 }
 
 // Opts a kernel in to `bytes` of dynamic shared memory, once per device.
@@ -894,9 +914,51 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
 }
 
 // ------------------------------------------------------------------ softmax loss, gradient
-// Bytes of one piece's g: a share of the 126 MB L2, so that the two products
-// that read it find it there.
-constexpr uint64_t kPieceBytes = 64ull << 20;
+// Most bytes of a piece's g: enough columns that the products of a piece fill
+// the GPU for many rounds of tiles; a small part of all scores of a large call.
+constexpr uint64_t kPieceBytes = 256ull << 20;
+
+struct GradPlan {
+    uint64_t width;      // columns of a piece, the last one narrower
+    Plan g, dx, dw, dw_last;
+};
+
+Plan plan_grad_tiles(const Shape& s)
+{
+    const Plan q = tiles_of(s, 2, 256);
+    return uint64_t(q.tiles_m) * q.tiles_n * 2 >= sm_count() * 3ull / 4 ? q : tiles_of(s, 1, 128);
+}
+
+// Pieces: as few as their bytes allow, or a few more where that evens out the
+// rounds of the three products (looked for only in calls of 0.2 ms and more).
+GradPlan plan_grad(uint64_t m, uint64_t k, uint64_t n, int dtype)
+{
+    const uint32_t planes = planes_of(dtype), combos = planes == 3 ? 6 : 1;
+    const bool f32 = planes == 3, bf16 = dtype == KNNG_DTYPE_BF16;
+    const uint64_t widest = std::max<uint64_t>(2048, kPieceBytes / (2 * planes * m) / 256 * 256);
+    const uint64_t fewest = ceil_div(n, widest);
+    GradPlan best{};
+    double least = 0.0;
+    for (uint64_t pieces = fewest; pieces < fewest + 6; ++pieces) {
+        GradPlan p;
+        p.width = std::min(up(ceil_div(n, pieces), 256), n);
+        if (pieces > fewest && p.width < 2048) break;
+        const uint64_t count = ceil_div(n, p.width);
+        const Shape sg{m, p.width, k, combos, f32, bf16}, sx{m, k, p.width, combos, f32, bf16};
+        const Shape sw{p.width, k, m, combos, f32, bf16}, sl{n - (count - 1) * p.width, k, m, combos, f32, bf16};
+        p.g = plan_grad_tiles(sg);
+        p.dx = plan_product(sx);
+        p.dw = plan_product(sw);
+        p.dw_last = count > 1 ? plan_product(sl) : p.dw;
+        const double c = static_cast<double>(count) * (plan_cycles(p.g, sg) + plan_cycles(p.dx, sx) + plan_cycles(p.dw, sw));
+        if (least == 0.0 || c < least) {
+            least = c;
+            best = p;
+        }
+        if (least < 4e5) break;
+    }
+    return best;
+}
 
 knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_args& a, void* ws, uint64_t ws_bytes,
                                           cudaStream_t st, uint64_t* need)
@@ -914,20 +976,13 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     const uint32_t planes = planes_of(a.dtype);
     const uint32_t combos = planes == 3 ? 6 : 1;
     const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
-    // Columns per piece: whole tiles, at least 2048 so that each product fills the GPU, all pieces alike.
-    const uint64_t want = std::max<uint64_t>(2048, kPieceBytes / (2 * planes * a.m) / 256 * 256);
-    const uint64_t pieces = ceil_div(a.n, want);
-    const uint64_t width = up(ceil_div(a.n, pieces), 256);
-    const uint64_t gpitch = up(std::min(width, a.n), 64);
     const bool f32 = planes == 3;
-    const Shape sg{a.m, std::min(width, a.n), a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
-    const Shape sx{a.m, a.k, std::min(width, a.n), combos, f32, a.dtype == KNNG_DTYPE_BF16};
-    const Plan qx = plan_product(sx);
+    const GradPlan plan = plan_grad(a.m, a.k, a.n, a.dtype);
+    const uint64_t width = plan.width;
+    const uint64_t gpitch = up(width, 64);
+    const Plan& qx = plan.dx;
     const uint64_t xpart_rows = qx.split_rows, xpart_pitch = qx.part_pitch;
-    const auto dw_shape = [&](uint64_t cols) { return Shape{cols, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16}; };
-    const uint64_t last = a.n - (ceil_div(a.n, width) - 1) * width;
-    const Plan qw0 = plan_product(dw_shape(std::min(width, a.n))), qw1 = plan_product(dw_shape(last));
-    for (const Plan& q : {tiles_of(sg, 1, 128), qx, qw0, qw1}) KNNG_TRY(check_items(op, q));
+    for (const Plan& q : {plan.g, plan.dx, plan.dw, plan.dw_last}) KNNG_TRY(check_items(op, q));
     Carver c(ws);
     uint16_t* xs = c.take<uint16_t>(stage_elems(x, a.dtype));
     uint16_t* wst = needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
@@ -937,7 +992,7 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     float* rest = planes == 1 ? c.take<float>(a.m) : nullptr;
     uint16_t* g = c.take<uint16_t>(a.m * gpitch * planes);
     float* xpart = a.dx ? c.take<float>(qx.splits * xpart_rows * xpart_pitch) : nullptr;
-    const uint64_t wpart_elems = a.dw ? std::max(qw0.part_elems(), qw1.part_elems()) : 0;
+    const uint64_t wpart_elems = a.dw ? std::max(plan.dw.part_elems(), plan.dw_last.part_elems()) : 0;
     float* wpart = wpart_elems ? c.take<float>(wpart_elems) : nullptr;
     if (need) {
         *need = c.at;
@@ -967,8 +1022,8 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         const uint64_t cols = std::min(width, a.n - c0);
         const Operand wp{static_cast<const uint16_t*>(ow.ptr) + c0 * ow.ld, cols, ow.width, ow.ld, ow.plane};
         const Shape s1{a.m, cols, a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
-        Plan q1 = tiles_of(s1, 2, 256);
-        if (uint64_t(q1.tiles_m) * q1.tiles_n * 2 < sm_count() * 3ull / 4) q1 = tiles_of(s1, 1, 128);
+        const bool last = c0 + width >= a.n;
+        const Plan q1 = last ? plan_grad_tiles(s1) : plan.g;
         CUtensorMap ma, mb, mo;
         KNNG_TRY(operand_maps(q1, ox, wp, kKK, operand_type(a.dtype), &ma, &mb));
         ProductParams p = base_params(s1, q1, ox, wp, a.dtype, err);
@@ -990,8 +1045,8 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         KNNG_TRY(launch_any<kEpiGrad>(q1.cg, kKK, ma, mb, mo, mo, p, st));
         const Operand og{g, a.m, gwidth, gld, static_cast<uint32_t>(gpitch)};
         if (a.dw) {
-            const Shape sw = dw_shape(cols);
-            const Plan qw = plan_product(sw);
+            const Shape sw{cols, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16};
+            const Plan& qw = last && c0 > 0 ? plan.dw_last : plan.dw;
             Tail t{static_cast<uint8_t*>(a.dw) + c0 * a.k * e, a.k, a.dtype};
             t.alpha = 1.0f / gscale;
             t.alpha_dev = cmax;
