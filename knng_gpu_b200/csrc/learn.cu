@@ -191,30 +191,50 @@ struct RowLabels {
     uint32_t classes = 0;
 };
 
-knng_gpu_status stage(const Source& s, int dtype, uint16_t* dst, Operand* out, cudaStream_t st,
-                      const RowLabels& labels = RowLabels(), float* zero = nullptr)
+// The work of staging s at dst (none where dst is NULL).
+StageJob stage_job(const Source& s, int dtype, uint16_t* dst, const RowLabels& labels = RowLabels())
 {
-    const uint64_t pitch = stage_pitch(s.k, dtype);
-    const uint64_t blocks = std::min<uint64_t>(ceil_div(s.rows * (pitch / 8), 256), 148ull * 16);
-    if (dtype == KNNG_DTYPE_F32)
-        KNNG_TRY(launch(stage_rows_kernel<3>, dim3(static_cast<uint32_t>(blocks)), 256, 0, st, s.ptr, s.rows, s.k, s.ld,
-                        dst, pitch, labels.ptr, labels.i64, labels.classes, zero));
-    else
-        KNNG_TRY(launch(stage_rows_kernel<1>, dim3(static_cast<uint32_t>(blocks)), 256, 0, st, s.ptr, s.rows, s.k, s.ld,
-                        dst, pitch, labels.ptr, labels.i64, labels.classes, zero));
-    const uint32_t planes = planes_of(dtype);
-    *out = Operand{dst, s.rows, pitch * planes, pitch * planes, static_cast<uint32_t>(pitch)};
-    return KNNG_GPU_OK;
+    StageJob j = {};
+    if (!dst) return j;
+    j.x = s.ptr;
+    j.rows = s.rows;
+    j.k = static_cast<uint32_t>(s.k);
+    j.ld = s.ld;
+    j.out = dst;
+    j.pitch = static_cast<uint32_t>(stage_pitch(s.k, dtype));
+    j.labels = labels.ptr;
+    j.labels_i64 = labels.i64;
+    j.classes = labels.classes;
+    j.blocks = static_cast<uint32_t>(std::min<uint64_t>(ceil_div(s.rows * (j.pitch / 8), 256), 148ull * 16));
+    return j;
 }
 
-Operand direct(const Source& s) { return Operand{s.ptr, s.rows, s.k, s.ld, 0}; }
-
-// The operand as the product reads it: staged through `dst` where needed.
-knng_gpu_status operand(const Source& s, int dtype, uint16_t* dst, Operand* out, cudaStream_t st)
+// The operand as the product reads it: staged at dst, or as the caller has it.
+Operand operand(const Source& s, int dtype, const uint16_t* dst)
 {
-    if (needs_stage(s, dtype)) return stage(s, dtype, dst, out, st);
-    *out = direct(s);
-    return KNNG_GPU_OK;
+    if (!dst) return Operand{s.ptr, s.rows, s.k, s.ld, 0};
+    const uint64_t pitch = stage_pitch(s.k, dtype), width = pitch * planes_of(dtype);
+    return Operand{dst, s.rows, width, width, static_cast<uint32_t>(pitch)};
+}
+
+knng_gpu_status prepare(int dtype, const StageJob& a, const StageJob& b, const GradRowsJob& rows, cudaStream_t st)
+{
+    const uint32_t blocks = a.blocks + b.blocks + rows.blocks;
+    if (blocks == 0) return KNNG_GPU_OK;
+    return dtype == KNNG_DTYPE_F32 ? launch(prepare_kernel<3>, dim3(blocks), 256, 0, st, PrepareParams{a, b, rows})
+                                   : launch(prepare_kernel<1>, dim3(blocks), 256, 0, st, PrepareParams{a, b, rows});
+}
+
+knng_gpu_status finish(const SumsJob& sums, const JoinParams& a, const JoinParams& b, cudaStream_t st)
+{
+    const uint32_t blocks = sums.blocks + a.blocks + b.blocks;
+    if (blocks == 0) return KNNG_GPU_OK;
+    return launch(finish_kernel, dim3(blocks), 256, 0, st, FinishParams{sums, a, b});
+}
+
+uint32_t join_blocks(uint64_t m, uint64_t n)
+{
+    return static_cast<uint32_t>(std::min<uint64_t>(ceil_div(m * ceil_div(n, 4), 256), 148ull * 16));
 }
 
 // ------------------------------------------------------------------ product launches
@@ -467,11 +487,13 @@ struct Tail {
     int activation = KNNG_ACT_NONE;
     float alpha = 1.0f;
     const float* alpha_dev = nullptr;
+    uint32_t alpha_parts = 0;
 };
 
-// D = A B^T through the tail; `part` holds the pieces where the plan splits K.
+// D = A B^T through the tail; where the plan splits K, the pieces in `part` and
+// the work of joining them in *join.
 knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, const Operand& b, Layout lay, int dtype,
-                              const Tail& t, float* part, int* err, cudaStream_t st)
+                              const Tail& t, float* part, JoinParams* join, int* err, cudaStream_t st)
 {
     CUtensorMap ma, mb, mo, mp;
     KNNG_TRY(operand_maps(q, a, b, lay, operand_type(dtype), &ma, &mb));
@@ -483,7 +505,7 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
         p.split_rows = static_cast<uint32_t>(q.split_rows);
         KNNG_TRY(make_map(&mo, KNNG_DTYPE_F32, part, q.part_pitch, q.splits * q.split_rows, q.part_pitch, 32, 32));
         KNNG_TRY(launch_any<kEpiStore>(q.cg, lay, ma, mb, mo, mo, p, st));
-        JoinParams j = {};
+        JoinParams& j = *join;
         j.part = part;
         j.splits = q.splits;
         j.split_rows = q.split_rows;
@@ -492,6 +514,7 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
         j.n = static_cast<uint32_t>(s.n);
         j.alpha = t.alpha;
         j.alpha_dev = t.alpha_dev;
+        j.alpha_parts = t.alpha_parts;
         j.bias = t.bias;
         j.residual = t.residual;
         j.ldr = t.ldr;
@@ -502,8 +525,7 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
         j.out_type = t.out_type;
         j.pre = t.pre;
         j.ldp = t.ldp;
-        const uint64_t blocks = std::min<uint64_t>(ceil_div(s.m * ceil_div(s.n, 4), 256), 148ull * 16);
-        KNNG_TRY(launch(join_splits_kernel, dim3(static_cast<uint32_t>(blocks)), 256, 0, st, j));
+        j.blocks = join_blocks(s.m, s.n);
         return KNNG_GPU_OK;
     }
     p.out = t.out;
@@ -522,6 +544,7 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
     p.activation = t.activation;
     p.alpha = t.alpha;
     p.alpha_dev = t.alpha_dev;
+    p.alpha_parts = t.alpha_parts;
     mo = ma;
     mp = ma;
     if (p.out_tma) KNNG_TRY(make_map(&mo, t.out_type, t.out, s.n, s.m, t.ldo, 32, 32));
@@ -579,11 +602,17 @@ knng_gpu_status check_workspace(const char* op, const void* ws, uint64_t have, u
 // Few rows of x go to the skinny kernel, its shared memory permitting. Against
 // the product kernel (padded to 128 rows), a linear layer of 16 bf16 rows takes
 // 6.8 us instead of 7.5 at 960 -> 1024 and 43 instead of 47 at 960 -> 100,000;
-// of 32 rows 11.3 instead of 7.5 and 67 instead of 47.
-bool is_skinny(uint64_t m, uint64_t k, int dtype)
+// of 32 rows 11.3 instead of 7.5 and 67 instead of 47. Rows that would have to
+// be staged first (fp16 33 x 785 -> 300: 8.5 us instead of 10.9, in one launch
+// instead of two or three) go there up to 64, sixteen to a block, while w is
+// small enough to be read several times from L2.
+bool is_skinny(const Source& x, const Source& w, int dtype)
 {
-    return m <= kSkinnyRows && k <= kMaxWidth / 2 &&
-           up(m, 8) * skinny_pitch(static_cast<uint32_t>(k), dtype == KNNG_DTYPE_F32) <= kSkinnySmem;
+    if (x.k > kMaxWidth / 2 || up(std::min<uint64_t>(x.rows, kSkinnyRows), 8) *
+                                       skinny_pitch(static_cast<uint32_t>(x.k), dtype == KNNG_DTYPE_F32) > kSkinnySmem)
+        return false;
+    if (x.rows <= kSkinnyRows) return true;
+    return x.rows <= 4 * kSkinnyRows && w.rows * w.k <= (2ull << 20) && (needs_stage(x, dtype) || needs_stage(w, dtype));
 }
 
 struct SkinnyPlan {
@@ -607,7 +636,7 @@ knng_gpu_status launch_skinny_t(const SkinnyParams& p, uint32_t blocks, cudaStre
     constexpr auto* kern = skinny_kernel<TYPE, NT, EPI>;
     const uint32_t smem = NT * 8 * p.pitch;
     if (smem > 16 * 1024) KNNG_TRY(allow_smem<kern>(kSkinnySmem));
-    return launch(kern, dim3(blocks), 256, smem, st, p);
+    return launch(kern, dim3(blocks, (p.m + kSkinnyRows - 1) / kSkinnyRows), 256, smem, st, p);
 }
 
 template <int TYPE, int EPI>
@@ -656,7 +685,7 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     const Source x{a.x, a.m, a.k, a.ldx}, w{a.w, a.n, a.k, a.ldw};
     const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, a.out_dtype == KNNG_DTYPE_F32,
                   a.dtype == KNNG_DTYPE_BF16};
-    const bool skinny = is_skinny(a.m, a.k, a.dtype);
+    const bool skinny = is_skinny(x, w, a.dtype);
     const Plan q = skinny ? Plan{} : plan_product(s);
     if (skinny && need) return KNNG_GPU_OK;
     KNNG_TRY(check_items(op, q));
@@ -691,9 +720,7 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     }
     int* err;
     KNNG_TRY(take_error(&err));
-    Operand ox, ow;
-    KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
-    KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+    KNNG_TRY(prepare(a.dtype, stage_job(x, a.dtype, xs), stage_job(w, a.dtype, wst), GradRowsJob{}, st));
     Tail t{a.out, a.ldo, a.out_dtype};
     t.pre = a.pre;
     t.ldp = a.ldp;
@@ -702,7 +729,9 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     t.ldr = a.ldr;
     t.aux_type = a.dtype;
     t.activation = a.activation;
-    return product_store(s, q, ox, ow, kKK, a.dtype, t, part, err, st);
+    JoinParams join = {};
+    KNNG_TRY(product_store(s, q, operand(x, a.dtype, xs), operand(w, a.dtype, wst), kKK, a.dtype, t, part, &join, err, st));
+    return finish(SumsJob{}, join, JoinParams{}, st);
 }
 
 // ------------------------------------------------------------------ linear backward
@@ -762,8 +791,8 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
     uint16_t* xs = a.dw && needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
     uint16_t* wst = a.dx && needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
     float* sums = a.db ? c.take<float>(uint64_t(gy) * a.n) : nullptr;
-    const uint64_t part_elems = std::max(a.dx ? qx.part_elems() : 0, a.dw ? qw.part_elems() : 0);
-    float* part = part_elems ? c.take<float>(part_elems) : nullptr;
+    float* xpart = a.dx && qx.splits > 1 ? c.take<float>(qx.part_elems()) : nullptr;
+    float* wpart = a.dw && qw.splits > 1 ? c.take<float>(qw.part_elems()) : nullptr;
     if (need) {
         *need = c.at;
         return KNNG_GPU_OK;
@@ -778,6 +807,8 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
     KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
     int* err;
     KNNG_TRY(take_error(&err));
+    const StageJob stage_x = stage_job(x, a.dtype, xs), stage_w = stage_job(w, a.dtype, wst);
+    SumsJob db = {};
     if (make_dz || a.db) {
         SlopeParams p = {};
         p.dy = a.dy;
@@ -790,29 +821,26 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
         p.pitch = static_cast<uint32_t>(pitch);
         p.sums = sums;
         p.vec = tma_rows(a.dy, a.lddy, e) && (!slope || tma_rows(a.pre, a.ldp, e));
-        KNNG_TRY(launch_slope(p, a.activation, a.dtype, dim3(gx, gy), st));
-        if (a.db) {
-            KNNG_TRY(launch(join_sums_kernel, dim3(static_cast<uint32_t>(ceil_div(a.n, 32))), 256, 0, st, sums, gy, a.n,
-                            a.db, a.dtype));
-        }
+        p.gx = gx;
+        p.gy = gy;
+        p.a = stage_x;
+        p.b = stage_w;
+        KNNG_TRY(launch_slope(p, a.activation, a.dtype, dim3(gx * gy + stage_x.blocks + stage_w.blocks), st));
+        if (a.db) db = SumsJob{sums, gy, static_cast<uint32_t>(a.n), a.db, a.dtype, static_cast<uint32_t>(ceil_div(a.n, 32))};
+    } else {
+        KNNG_TRY(prepare(a.dtype, stage_x, stage_w, GradRowsJob{}, st));
     }
-    if (!products) return KNNG_GPU_OK;
-    Operand oz = direct(dy);
-    if (make_dz)
-        oz = Operand{dz, a.m, pitch * planes_of(a.dtype), pitch * planes_of(a.dtype), static_cast<uint32_t>(pitch)};
-    if (a.dx) {
-        Operand ow;
-        KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
-        Tail t{a.dx, a.k, a.dtype};
-        KNNG_TRY(product_store(sx, qx, oz, ow, kKMN, a.dtype, t, part, err, st));
-    }
-    if (a.dw) {
-        Operand ox;
-        KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
-        Tail t{a.dw, a.k, a.dtype};
-        KNNG_TRY(product_store(sw, qw, oz, ox, kMNMN, a.dtype, t, part, err, st));
-    }
-    return KNNG_GPU_OK;
+    const Operand oz = make_dz ? Operand{dz, a.m, pitch * planes_of(a.dtype), pitch * planes_of(a.dtype),
+                                         static_cast<uint32_t>(pitch)}
+                               : operand(dy, a.dtype, nullptr);
+    JoinParams join_x = {}, join_w = {};
+    if (a.dx)
+        KNNG_TRY(product_store(sx, qx, oz, operand(w, a.dtype, wst), kKMN, a.dtype, Tail{a.dx, a.k, a.dtype}, xpart, &join_x,
+                               err, st));
+    if (a.dw)
+        KNNG_TRY(product_store(sw, qw, oz, operand(x, a.dtype, xs), kMNMN, a.dtype, Tail{a.dw, a.k, a.dtype}, wpart,
+                               &join_w, err, st));
+    return finish(db, join_x, join_w, st);
 }
 
 // ------------------------------------------------------------------ softmax loss
@@ -856,7 +884,7 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     const Shape s{a.m, a.n, a.k, a.dtype == KNNG_DTYPE_F32 ? 6u : 1u, true, a.dtype == KNNG_DTYPE_BF16};
     // Pairs unless they would leave SMs idle; then the columns are cut so that
     // (row tile, piece) items fill the units in whole rounds.
-    const bool skinny = is_skinny(a.m, a.k, a.dtype);
+    const bool skinny = is_skinny(x, w, a.dtype);
     const SkinnyPlan sq = plan_skinny(a.n, a.k);
     Plan q = tiles_of(s, 2, 256);
     if (s.m <= 128 || uint64_t(q.tiles_m) * q.tiles_n < sm_count() / 2) q = tiles_of(s, 1, 128);
@@ -889,9 +917,8 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     } else {
         int* err;
         KNNG_TRY(take_error(&err));
-        Operand ox, ow;
-        KNNG_TRY(operand(x, a.dtype, xs, &ox, st));
-        KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
+        KNNG_TRY(prepare(a.dtype, stage_job(x, a.dtype, xs), stage_job(w, a.dtype, wst), GradRowsJob{}, st));
+        const Operand ox = operand(x, a.dtype, xs), ow = operand(w, a.dtype, wst);
         CUtensorMap ma, mb;
         KNNG_TRY(operand_maps(q, ox, ow, kKK, operand_type(a.dtype), &ma, &mb));
         ProductParams p = base_params(s, q, ox, ow, a.dtype, err);
@@ -988,7 +1015,8 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     uint16_t* wst = needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;
     float* coef = c.take<float>(a.m);
     float* lse2 = c.take<float>(a.m);
-    float* cmax = c.take<float>(1);
+    const uint32_t row_blocks = static_cast<uint32_t>(std::min<uint64_t>(ceil_div(a.m, 256), 148));
+    float* cmax = c.take<float>(row_blocks);
     float* rest = planes == 1 ? c.take<float>(a.m) : nullptr;
     uint16_t* g = c.take<uint16_t>(a.m * gpitch * planes);
     float* xpart = a.dx ? c.take<float>(qx.splits * xpart_rows * xpart_pitch) : nullptr;
@@ -1009,16 +1037,16 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     int* err;
     KNNG_TRY(take_error(&err));
     const RowLabels labels{a.labels, a.labels_i64, static_cast<uint32_t>(a.n)};
-    Operand ox, ow;
-    KNNG_TRY(stage(x, a.dtype, xs, &ox, st, labels, cmax));
-    KNNG_TRY(operand(w, a.dtype, wst, &ow, st));
-    KNNG_TRY(launch(grad_rows_kernel, dim3(static_cast<uint32_t>(std::min<uint64_t>(ceil_div(a.m, 256), 148))), 256, 0,
-                    st, a.dloss, a.lse, a.m, a.scale, a.labels, a.labels_i64, a.n, coef, lse2,
-                    reinterpret_cast<uint32_t*>(cmax)));
+    const GradRowsJob rows{a.dloss, a.lse, a.m, a.scale, a.labels, a.labels_i64, static_cast<uint32_t>(a.n), coef, lse2,
+                           cmax, row_blocks};
+    KNNG_TRY(prepare(a.dtype, stage_job(x, a.dtype, xs, labels), stage_job(w, a.dtype, wst), rows, st));
+    const Operand ox = operand(x, a.dtype, xs), ow = operand(w, a.dtype, wst);
     // fp16 holds 2^14 g / max |dloss scale|: |g| <= 1 there, and the smallest
     // normal value 6e-5 then stands for 4e-9 instead of losing every p below it.
     const float gscale = a.dtype == KNNG_DTYPE_F16 ? 16384.0f : 1.0f;
+    JoinParams join_w = {};
     for (uint64_t c0 = 0; c0 < a.n; c0 += width) {
+        join_w = JoinParams{};
         const uint64_t cols = std::min(width, a.n - c0);
         const Operand wp{static_cast<const uint16_t*>(ow.ptr) + c0 * ow.ld, cols, ow.width, ow.ld, ow.plane};
         const Shape s1{a.m, cols, a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
@@ -1035,6 +1063,7 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         p.lse2 = lse2;
         p.coef = coef;
         p.alpha_dev = cmax;
+        p.alpha_parts = row_blocks;
         p.grad_scale = gscale;
         p.grad_planes = planes;
         p.label_rest = rest;
@@ -1050,7 +1079,10 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
             Tail t{static_cast<uint8_t*>(a.dw) + c0 * a.k * e, a.k, a.dtype};
             t.alpha = 1.0f / gscale;
             t.alpha_dev = cmax;
-            KNNG_TRY(product_store(sw, qw, og, ox, kMNMN, a.dtype, t, wpart, err, st));
+            t.alpha_parts = row_blocks;
+            KNNG_TRY(product_store(sw, qw, og, ox, kMNMN, a.dtype, t, wpart, &join_w, err, st));
+            // The last piece's joins wait for dx.
+            if (!last) KNNG_TRY(finish(SumsJob{}, join_w, JoinParams{}, st));
         }
         if (a.dx) {
             // Pieces add up in fp32: the first one stores, the others add.
@@ -1070,8 +1102,8 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
             KNNG_TRY(launch_any<kEpiStore>(qp.cg, kKMN, mga, mwb, mx, mx, px, st));
         }
     }
+    JoinParams j = {};
     if (a.dx) {
-        JoinParams j = {};
         j.part = xpart;
         j.splits = qx.splits;
         j.split_rows = xpart_rows;
@@ -1080,6 +1112,7 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         j.n = static_cast<uint32_t>(a.k);
         j.alpha = 1.0f / gscale;
         j.alpha_dev = cmax;
+        j.alpha_parts = row_blocks;
         j.out = a.dx;
         j.ldo = a.k;
         j.out_type = a.dtype;
@@ -1093,10 +1126,9 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         j.w = a.w;
         j.ldw = a.ldw;
         j.w_type = a.dtype;
-        const uint64_t blocks = std::min<uint64_t>(ceil_div(a.m * ceil_div(a.k, 4), 256), 148ull * 16);
-        KNNG_TRY(launch(join_splits_kernel, dim3(static_cast<uint32_t>(blocks)), 256, 0, st, j));
+        j.blocks = join_blocks(a.m, a.k);
     }
-    return KNNG_GPU_OK;
+    return finish(SumsJob{}, join_w, j, st);
 }
 
 // No exception leaves a C entry point.

@@ -7,54 +7,61 @@
 
 namespace knng_b200 {
 
-// Rows as 16-bit operands: `planes` = 1 copies 16-bit rows to a pitch that TMA
-// can read, 3 splits fp32 values into bf16 parts x = h + m + l (each rounded to
-// nearest from what is left; a finite value whose rounding would overflow is
-// truncated). Columns past k are zeros. Rows without a label are zeros when
-// labels are given. One thread per 8 columns. Also clears *zero, if given, for
-// the kernel after it.
+// Rows that become 16-bit operands.
+struct StageJob {
+    const void* x;
+    uint64_t rows;
+    uint32_t k;
+    uint64_t ld;
+    uint16_t* out;
+    uint32_t pitch;       // columns of a plane of out, a multiple of 8
+    const void* labels;   // where given, rows without a label become zeros
+    int labels_i64;
+    uint32_t classes;
+    uint32_t blocks;      // of the launch that work on it (0: nothing to do)
+};
+
+// One plane copies 16-bit rows to a pitch that TMA can read, three split fp32
+// values into bf16 parts x = h + m + l (each rounded to nearest from what is
+// left; a finite value whose rounding would overflow is truncated). Columns
+// past k are zeros. One thread per 8 columns.
 template <int PLANES>
-__global__ void __launch_bounds__(256) stage_rows_kernel(const void* __restrict__ x, uint64_t rows, uint32_t k,
-                                                         uint64_t ld, uint16_t* __restrict__ out, uint32_t pitch,
-                                                         const void* labels, int labels_i64, uint32_t classes,
-                                                         float* zero)
+__device__ void stage_rows(const StageJob& p, uint32_t block)
 {
-    previous_done();
-    if (zero && blockIdx.x == 0 && threadIdx.x == 0) *zero = 0.0f;
-    const uint32_t groups = pitch / 8;
-    const uint64_t total = rows * groups;
-    for (uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const uint32_t groups = p.pitch / 8;
+    const uint64_t total = p.rows * groups;
+    for (uint64_t i = block * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(p.blocks) * 256) {
         const uint64_t r = i / groups;
         const uint32_t c0 = static_cast<uint32_t>(i - r * groups) * 8;
-        const bool keep = !labels || load_label(labels, labels_i64, r, classes) >= 0;
+        const bool keep = !p.labels || load_label(p.labels, p.labels_i64, r, p.classes) >= 0;
         if constexpr (PLANES == 1) {
-            const uint16_t* src = static_cast<const uint16_t*>(x) + r * ld;
+            const uint16_t* src = static_cast<const uint16_t*>(p.x) + r * p.ld;
             uint32_t w[4];
-            if (keep && c0 + 8 <= k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
+            if (keep && c0 + 8 <= p.k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
                 const uint4 q = *reinterpret_cast<const uint4*>(src + c0);
                 w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t a = keep && c0 + 2 * j < k ? src[c0 + 2 * j] : 0u;
-                    const uint32_t b = keep && c0 + 2 * j + 1 < k ? src[c0 + 2 * j + 1] : 0u;
+                    const uint32_t a = keep && c0 + 2 * j < p.k ? src[c0 + 2 * j] : 0u;
+                    const uint32_t b = keep && c0 + 2 * j + 1 < p.k ? src[c0 + 2 * j + 1] : 0u;
                     w[j] = a | (b << 16);
                 }
             }
-            *reinterpret_cast<uint4*>(out + r * pitch + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(p.out + r * p.pitch + c0) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
-            const float* src = static_cast<const float*>(x) + r * ld;
+            const float* src = static_cast<const float*>(p.x) + r * p.ld;
             float v[8];
-            if (keep && c0 + 8 <= k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
+            if (keep && c0 + 8 <= p.k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
                 const float4 a = *reinterpret_cast<const float4*>(src + c0);
                 const float4 b = *reinterpret_cast<const float4*>(src + c0 + 4);
                 v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
                 v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = keep && c0 + j < k ? src[c0 + j] : 0.0f;
+                for (int j = 0; j < 8; ++j) v[j] = keep && c0 + j < p.k ? src[c0 + j] : 0.0f;
             }
-            uint16_t* dst = out + r * (3ull * pitch) + c0;
+            uint16_t* dst = p.out + r * (3ull * p.pitch) + c0;
 #pragma unroll
             for (int plane = 0; plane < 3; ++plane) {
                 uint32_t w[4];
@@ -73,7 +80,7 @@ __global__ void __launch_bounds__(256) stage_rows_kernel(const void* __restrict_
                     }
                     w[j] = h2;
                 }
-                *reinterpret_cast<uint4*>(dst + uint64_t(plane) * pitch) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(dst + uint64_t(plane) * p.pitch) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }
@@ -87,7 +94,8 @@ struct JoinParams {
     uint64_t m;
     uint32_t n;
     float alpha;
-    const float* alpha_dev;
+    const float* alpha_dev;  // the largest of alpha_parts values
+    uint32_t alpha_parts;
     const void* bias;
     const void* residual;
     uint64_t ldr;
@@ -105,16 +113,16 @@ struct JoinParams {
     const void* w;
     uint64_t ldw;
     int w_type;
+    uint32_t blocks;        // of the launch that work on it (0: nothing to do)
 };
 
 // The pieces of a split product, summed in order, and the linear epilogue.
-__global__ void __launch_bounds__(256) join_splits_kernel(const JoinParams p)
+__device__ void join_splits(const JoinParams& p, uint32_t block)
 {
-    previous_done();
     const uint32_t groups = (p.n + 3) / 4;
     const uint64_t total = p.m * groups;
-    const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
-    for (uint64_t i = blockIdx.x * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+    const float alpha = p.alpha_dev ? p.alpha * warp_largest(p.alpha_dev, p.alpha_parts) : p.alpha;
+    for (uint64_t i = block * uint64_t(256) + threadIdx.x; i < total; i += uint64_t(p.blocks) * 256) {
         const uint64_t r = i / groups;
         const uint32_t c = static_cast<uint32_t>(i - r * groups) * 4;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -208,25 +216,61 @@ __global__ void __launch_bounds__(256) join_softmax_kernel(const float2* __restr
 }
 
 // Per row of the gradient: coef = dloss scale and lse in base 2 (both 0 for a
-// row without a label), and the largest finite |coef| as float bits (a maximum
-// does not depend on the order of the atomics).
-__global__ void __launch_bounds__(256) grad_rows_kernel(const float* __restrict__ dloss, const float* __restrict__ lse,
-                                                        uint64_t m, float scale, const void* labels, int labels_i64,
-                                                        uint32_t classes, float* __restrict__ coef,
-                                                        float* __restrict__ lse2, uint32_t* cmax)
+// row without a label), and for each block of rows the largest finite |coef|.
+struct GradRowsJob {
+    const float* dloss;
+    const float* lse;
+    uint64_t m;
+    float scale;
+    const void* labels;
+    int labels_i64;
+    uint32_t classes;
+    float* coef;
+    float* lse2;
+    float* largest;   // [blocks]
+    uint32_t blocks;  // of the launch that work on it (0: nothing to do)
+};
+
+__device__ __forceinline__ void grad_rows(const GradRowsJob& p, uint32_t block)
 {
-    previous_done();
+    __shared__ float warps[8];
     float big = 0.0f;
-    for (uint64_t r = blockIdx.x * uint64_t(256) + threadIdx.x; r < m; r += uint64_t(gridDim.x) * 256) {
-        const bool has = load_label(labels, labels_i64, r, classes) >= 0;
-        const float c = has ? dloss[r] * scale : 0.0f;
-        coef[r] = c;
-        lse2[r] = has ? lse[r] * 1.44269504f : 0.0f;
+    for (uint64_t r = block * uint64_t(256) + threadIdx.x; r < p.m; r += uint64_t(p.blocks) * 256) {
+        const bool has = load_label(p.labels, p.labels_i64, r, p.classes) >= 0;
+        const float c = has ? p.dloss[r] * p.scale : 0.0f;
+        p.coef[r] = c;
+        p.lse2[r] = has ? p.lse[r] * 1.44269504f : 0.0f;
         if (isfinite(c)) big = fmaxf(big, fabsf(c));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
-    if ((threadIdx.x & 31) == 0 && big > 0.0f) atomicMax(cmax, __float_as_uint(big));
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) big = fmaxf(big, warps[w]);
+        p.largest[block] = big;
+    }
+}
+
+// What comes before the products, in one launch: up to two matrices to stage,
+// the rows of the gradient. Blocks are dealt out in that order.
+struct PrepareParams {
+    StageJob a, b;
+    GradRowsJob rows;
+};
+
+template <int PLANES>
+__global__ void __launch_bounds__(256) prepare_kernel(const PrepareParams p)
+{
+    previous_done();
+    uint32_t block = blockIdx.x;
+    if (block < p.a.blocks) {
+        stage_rows<PLANES>(p.a, block);
+    } else if ((block -= p.a.blocks) < p.b.blocks) {
+        stage_rows<PLANES>(p.b, block);
+    } else {
+        grad_rows(p.rows, block - p.b.blocks);
+    }
 }
 
 constexpr int kSlopeBlocks = 4;  // per SM, all resident
@@ -240,8 +284,10 @@ struct SlopeParams {
     uint32_t n;
     uint16_t* out;        // dz as 16-bit operands (may be NULL: column sums only)
     uint32_t pitch;       // columns of a plane of out
-    float* sums;          // [gridDim.y][n] column sums (may be NULL)
+    float* sums;          // [gy][n] column sums (may be NULL)
     int vec;              // rows of dy and pre allow 16-byte loads
+    uint32_t gx, gy;      // blocks over columns and rows
+    StageJob a, b;        // matrices that the products after it need staged
 };
 
 // 8 consecutive values as they lie; those past `left` are zeros.
@@ -292,9 +338,18 @@ __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopePar
     constexpr int kPlanes = TYPE == kF32 ? 3 : 1;
     __shared__ float total[8][256];
     previous_done();
+    if (blockIdx.x >= p.gx * p.gy) {
+        const uint32_t block = blockIdx.x - p.gx * p.gy;
+        if (block < p.a.blocks)
+            stage_rows<kPlanes>(p.a, block);
+        else
+            stage_rows<kPlanes>(p.b, block - p.a.blocks);
+        return;
+    }
+    const uint32_t bx = blockIdx.x % p.gx, by = blockIdx.x / p.gx;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t c0 = blockIdx.x * 256 + lane * 8;
-    const uint64_t r0 = p.m * blockIdx.y / gridDim.y, r1 = p.m * (blockIdx.y + 1) / gridDim.y;
+    const uint32_t c0 = bx * 256 + lane * 8;
+    const uint64_t r0 = p.m * by / p.gy, r1 = p.m * (by + 1) / p.gy;
     const uint32_t left = c0 < p.n ? p.n - c0 : 0;
     const bool whole = p.vec && left >= 8;
     uint64_t acc[4] = {0, 0, 0, 0};
@@ -357,33 +412,58 @@ __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopePar
             total[warp][lane * 8 + 2 * j + 1] = f.y;
         }
         __syncthreads();
-        const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+        const uint32_t c = bx * 256 + threadIdx.x;
         if (c < p.n) {
             float s = 0.0f;
             for (int w = 0; w < 8; ++w) s += total[w][threadIdx.x];
-            p.sums[uint64_t(blockIdx.y) * p.n + c] = s;
+            p.sums[uint64_t(by) * p.n + c] = s;
         }
     }
 }
 
 // Column sums of [rows][n] partial sums: 32 columns per block, 8 row groups
 // added in order.
-__global__ void __launch_bounds__(256) join_sums_kernel(const float* __restrict__ sums, uint32_t rows, uint32_t n,
-                                                        void* out, int type)
+struct SumsJob {
+    const float* sums;
+    uint32_t rows, n;
+    void* out;
+    int type;
+    uint32_t blocks;  // of the launch that work on it (0: nothing to do)
+};
+
+__device__ __forceinline__ void join_sums(const SumsJob& p, uint32_t block)
 {
     __shared__ float part[8][32];
-    previous_done();
     const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t c = blockIdx.x * 32 + lane;
+    const uint32_t c = block * 32 + lane;
     float s = 0.0f;
-    if (c < n)
-        for (uint32_t r = g; r < rows; r += 8) s += sums[uint64_t(r) * n + c];
+    if (c < p.n)
+        for (uint32_t r = g; r < p.rows; r += 8) s += p.sums[uint64_t(r) * p.n + c];
     part[g][lane] = s;
     __syncthreads();
-    if (g == 0 && c < n) {
+    if (g == 0 && c < p.n) {
         float t = 0.0f;
         for (int i = 0; i < 8; ++i) t += part[i][lane];
-        store_elem(out, c, t, type);
+        store_elem(p.out, c, t, p.type);
+    }
+}
+
+// What comes after the products, in one launch.
+struct FinishParams {
+    SumsJob sums;
+    JoinParams a, b;
+};
+
+__global__ void __launch_bounds__(256) finish_kernel(const FinishParams p)
+{
+    previous_done();
+    uint32_t block = blockIdx.x;
+    if (block < p.sums.blocks) {
+        join_sums(p.sums, block);
+    } else if ((block -= p.sums.blocks) < p.a.blocks) {
+        join_splits(p.a, block);
+    } else {
+        join_splits(p.b, block - p.a.blocks);
     }
 }
 

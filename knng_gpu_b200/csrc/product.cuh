@@ -78,7 +78,8 @@ struct ProductParams {
     int bias_vec, residual_vec;    // they allow 16-byte loads
     int activation;
     float alpha;                   // D is scaled by alpha * *alpha_dev
-    const float* alpha_dev;
+    const float* alpha_dev;        // the largest of alpha_parts values
+    uint32_t alpha_parts;
     // softmax and gradient
     float scale2;                  // scale * log2(e)
     const void* labels;            // class of each row, int64 or int32; outside [0, classes) where it has none
@@ -397,6 +398,16 @@ __device__ __forceinline__ int32_t load_label(const void* labels, int i64, uint6
     return y >= 0 && y < static_cast<int64_t>(classes) ? static_cast<int32_t>(y) : -1;
 }
 
+// The largest of n values >= 0 (0 if there are none), in every lane of a warp.
+__device__ __forceinline__ float warp_largest(const float* v, uint32_t n)
+{
+    float big = 0.0f;
+    for (uint32_t i = threadIdx.x & 31; i < n; i += 32) big = fmaxf(big, v[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
+    return big;
+}
+
 // ---------------------------------------------------------------- schedule
 struct Item {
     uint32_t tm, n0, n1, p0, p1, split, segment;  // row tile, column tiles, K pieces
@@ -461,7 +472,12 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                    const ProductParams p)
 {
     constexpr int EW = pk_epi_warps(CG, EPI, LONG);
-    constexpr int kGroups = EW / 4;          // warps that share a quarter of the rows
+    // Softmax with 16 warps: eight for each of the two accumulator buffers, so
+    // that one half exponentiates while the other waits, loads and looks for
+    // maxima (2048 x 128 against a million rows: 583 -> 558 us; stores gain
+    // nothing, a gelu layer of 100,000 x 784 -> 1024 took 203 us instead of 189).
+    constexpr int kSets = EPI == kEpiSoftmax && EW == 16 ? 2 : 1;
+    constexpr int kGroups = EW / 4 / kSets;  // warps that share a quarter of the rows of a tile
     constexpr uint32_t kBufCols = 128 * CG;  // TMEM columns of an accumulator buffer
     constexpr uint32_t kTmemCols = 2 * kBufCols;
     const uint32_t bn_tile = p.tile_n;
@@ -492,7 +508,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], CG * EW);
+            mbar_init(&tempty[b], CG * EW / kSets);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -695,7 +711,8 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pk_epi_regs(EW)));
         const int e = warp - 4;
         const uint32_t quarter = warp & 3;
-        const uint32_t group = e >> 2;
+        const uint32_t group = (e >> 2) % kGroups;
+        const uint32_t set = (e >> 2) / kGroups;
         // 32-column chunks of this warp: number group, group + kGroups, ...
         constexpr int kMaxChunks = 4 * CG / kGroups;
         constexpr uint32_t kStep = 32 * kGroups;  // columns from one to the next
@@ -848,6 +865,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
             return true;
         };
 
+        const float largest = p.alpha_dev ? warp_largest(p.alpha_dev, p.alpha_parts) : 1.0f;
         for (uint32_t it = unit; ok && it < p.items; it += units) {
             const Item t = decode_item<EPI>(p, it);
             const uint32_t row0 = t.tm * (128 * CG) + cta * 128 + quarter * 32;
@@ -855,7 +873,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
             const bool live = row < p.m;
 
             if constexpr (EPI == kEpiStore) {
-                const float alpha = p.alpha_dev ? p.alpha * *p.alpha_dev : p.alpha;
+                const float alpha = p.alpha * largest;
                 const uint32_t col_base = t.n0 * bn_tile + group * 32;
                 const uint32_t out_row0 = row0 + t.split * p.split_rows;
                 ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
@@ -1009,24 +1027,30 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         for (int i = 0; i < kMaxChunks; i += 2) soft(sums + 32 * i, tn * bn_tile + group * 32 + i * kStep);
                     }
                 } else {
-                    static_assert(LONG || kMaxChunks == 2, "one batch");
                     for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
+                        if (kSets == 2 && (acc & 1u) != set) {
+                            ++acc;
+                            continue;
+                        }
                         uint32_t buf;
                         ok = wait_acc(buf);
                         if (!ok) break;
-                        float v[64];
-                        issue(buf, 0, v);
-                        issue(buf, 1, v + 32);
-                        arrived(v);
-                        tie32(reinterpret_cast<int32_t*>(v + 32));
-                        release(buf);
-                        soft(v, tn * bn_tile + group * 32);
+#pragma unroll 1
+                        for (int i = 0; i < kMaxChunks; i += 2) {
+                            float v[64];
+                            issue(buf, i, v);
+                            issue(buf, i + 1, v + 32);
+                            arrived(v);
+                            tie32(reinterpret_cast<int32_t*>(v + 32));
+                            if (i + 2 == kMaxChunks) release(buf);
+                            soft(v, tn * bn_tile + group * 32 + i * kStep);
+                        }
                     }
                 }
-                if (ok && live) p.part[uint64_t(kGroups * t.segment + group) * p.m + row] = make_float2(top, sum);
+                if (ok && live) p.part[uint64_t(EW / 4 * t.segment + (e >> 2)) * p.m + row] = make_float2(top, sum);
             } else {
                 const float lse2 = live ? p.lse2[row] : 0.0f;
-                const float cmax_inv = *p.alpha_dev > 0.0f ? 1.0f / *p.alpha_dev : 0.0f;
+                const float cmax_inv = largest > 0.0f ? 1.0f / largest : 0.0f;
                 const float coef = live ? p.coef[row] * cmax_inv * p.grad_scale : 0.0f;
                 // Column of the row's class here; negative where it has none or an earlier piece holds it.
                 int32_t label = live ? load_label(p.labels, p.labels_i64, row, p.classes) : -1;

@@ -1,4 +1,4 @@
-// skinny.cuh -- x w^T for few rows of x (one to 16), with the linear
+// skinny.cuh -- x w^T for few rows of x (16 to a block), with the linear
 // epilogue or the softmax pieces of product.cuh's kernel.
 //
 // Such a call reads w once and does little else, so it is bound by HBM on a
@@ -21,7 +21,7 @@
 
 namespace knng_b200 {
 
-constexpr int kSkinnyRows = 16;         // most rows of x
+constexpr int kSkinnyRows = 16;         // rows of x a block takes
 constexpr uint32_t kSkinnySmem = 96 * 1024;  // most shared memory for x
 
 struct SkinnyParams {
@@ -113,6 +113,8 @@ __device__ __forceinline__ void load_w(const SkinnyParams& p, uint32_t row, uint
 template <int TYPE, int NT, int EPI>
 __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
 {
+    const uint32_t token0 = blockIdx.y * kSkinnyRows;
+    const uint32_t tokens = min(p.m - token0, static_cast<uint32_t>(kSkinnyRows));
     constexpr int kWords = TYPE == kF32 ? 8 : 4;  // of 8 values
     extern __shared__ __align__(16) uint8_t xs[];
     __shared__ float red[8][NT * 4][32];
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
     for (uint32_t i = threadIdx.x; i < NT * 8 * octets; i += 256) {
         const uint32_t r = i / octets, c = (i - r * octets) * 8;
         uint32_t v[kWords];
-        load8_words<TYPE>(p.x, r * p.ldx + c, r < p.m && c < p.k ? p.k - c : 0u, p.x_vec, v);
+        load8_words<TYPE>(p.x, (token0 + r) * p.ldx + c, r < tokens && c < p.k ? p.k - c : 0u, p.x_vec, v);
 #pragma unroll
         for (int q = 0; q < kWords; q += 4)
             *reinterpret_cast<uint4*>(xs + r * p.pitch + c * (kWords / 2) + q * 4) =
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
             const uint32_t token = (i >> 1) * 8 + 2 * t + (i & 1);
             top[i] = -INFINITY;
             sum[i] = 0.0f;
-            label[i] = token < p.m ? load_label(p.labels, p.labels_i64, token, p.n) : -1;
+            label[i] = token < tokens ? load_label(p.labels, p.labels_i64, token0 + token, p.n) : -1;
         }
     }
 
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                     if (s + u * p.ksplit >= steps) break;
 #pragma unroll
                     for (int q = 0; q < NT * 8; ++q) {
-                        if (q >= static_cast<int>(p.m)) break;
+                        if (q >= static_cast<int>(tokens)) break;
                         const float4* b = reinterpret_cast<const float4*>(xs + q * p.pitch + (s + u * p.ksplit) * 128 + t * 32);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
             }
 #pragma unroll
             for (int q = 0; q < NT * 8; ++q) {
-                if (q >= static_cast<int>(p.m)) break;
+                if (q >= static_cast<int>(tokens)) break;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float v = f[r][q];
@@ -252,9 +254,10 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
             for (int q = 0; q < NT; ++q)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint64_t token = q * 8 + 2 * t + (j & 1);
+                    const uint32_t here = q * 8 + 2 * t + (j & 1);
+                    const uint64_t token = token0 + here;
                     const uint32_t col = r0 + 8 * (j >> 1);
-                    if (token >= p.m || col >= p.n) continue;
+                    if (here >= tokens || col >= p.n) continue;
                     float z = acc[q][j];
                     if (p.bias) z += load_elem(p.bias, col, TYPE);
                     if (p.pre) store_elem(p.pre, token * p.ldp + col, z, TYPE);
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                     const uint32_t col = r0 + 8 * h;
                     v[h] = acc[i >> 1][2 * h + (i & 1)];
                     if (static_cast<int32_t>(col) == label[i]) {
-                        p.label_dot[(i >> 1) * 8 + 2 * t + (i & 1)] = v[h];
+                        p.label_dot[token0 + (i >> 1) * 8 + 2 * t + (i & 1)] = v[h];
                         v[h] = -INFINITY;  // its term is added by the join
                     }
                     if (col >= p.n) v[h] = -INFINITY;
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
             if (g == 0) parts[warp * NT * 8 + (i >> 1) * 8 + 2 * t + (i & 1)] = make_float2(top[i], sum[i]);
         }
         __syncthreads();
-        if (threadIdx.x < p.m) {
+        if (threadIdx.x < tokens) {
             float m0 = -INFINITY, s = 0.0f;
             for (int w = 0; w < 8; ++w) {
                 const float2 q = parts[w * NT * 8 + threadIdx.x];
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                 s = s * exp2_approx(m0 - base) + q.y * exp2_approx(q.x - base);
                 m0 = now;
             }
-            p.part[uint64_t(blockIdx.x) * p.m + threadIdx.x] = make_float2(m0, s);
+            p.part[uint64_t(blockIdx.x) * p.m + token0 + threadIdx.x] = make_float2(m0, s);
         }
     }
 }
