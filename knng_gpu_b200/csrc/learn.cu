@@ -140,6 +140,7 @@ knng_gpu_status encode_fn(EncodeTiledFn* out)
 knng_gpu_status make_map(CUtensorMap* map, int type, const void* base, uint64_t width, uint64_t rows, uint64_t ld,
                          uint32_t box_w, uint32_t box_h)
 {
+    if (!base) return fail(KNNG_GPU_INVALID_ARGUMENT, "knng::gpu: a matrix of a product is NULL");
     EncodeTiledFn enc;
     KNNG_TRY(encode_fn(&enc));
     const uint32_t e = elem_bytes(type);
@@ -306,11 +307,12 @@ double plan_cycles(const Plan& q, const Shape& s)
 // 64 columns up, the K loop whole or cut into 2, 3, 4, 6, 8, ... splits of at
 // least four K blocks: where the tiles leave units idle, up to as many as fill
 // them; where they do not, up to eight, to even out the last round.
-Plan search_plan(const Shape& s)
+Plan search_plan(const Shape& s, int only_cg)
 {
     Plan best;
     double least = 0.0;
     for (int cg = 2; cg >= 1; --cg) {
+        if (only_cg && cg != only_cg) continue;
         for (uint32_t tile_n = 128 * cg; tile_n >= 64u * cg; tile_n -= 32) {
             Plan q = tiles_of(s, cg, tile_n);
             const uint32_t whole = q.piece;
@@ -336,21 +338,38 @@ Plan search_plan(const Shape& s)
 }
 
 // The search takes some microseconds of host time: a thread keeps the plans of
-// the shapes it met last.
-Plan plan_product(const Shape& s)
+// the shapes it met last. `cg` 1 or 2 asks for that kind of tile, 0 for either.
+Plan plan_product(const Shape& s, int cg = 0)
 {
     struct Entry {
         Shape s;
+        int cg;
         Plan q;
     };
-    thread_local Entry kept[64] = {};
+    thread_local Entry kept[128] = {};
     const uint64_t key = (s.m * 0x9E3779B97F4A7C15ull + s.n) * 0xC2B2AE3D27D4EB4Full + s.k * 0x165667B19E3779F9ull +
-                         s.combos * 4 + s.precise * 2 + s.bf16;
-    Entry& e = kept[(key ^ (key >> 29)) & 63];
+                         s.combos * 16 + cg * 4 + s.precise * 2 + s.bf16;
+    Entry& e = kept[(key ^ (key >> 29)) & 127];
     if (e.s.m != s.m || e.s.n != s.n || e.s.k != s.k || e.s.combos != s.combos || e.s.precise != s.precise ||
-        e.s.bf16 != s.bf16)
-        e = Entry{s, search_plan(s)};
+        e.s.bf16 != s.bf16 || e.cg != cg)
+        e = Entry{s, cg, search_plan(s, cg)};
     return e.q;
+}
+
+// Plans of two products of one backward pass, and whether they run in one
+// launch: that saves a launch and half-empty rounds where they are short
+// (gradients of 1537 x 960 -> 300: 26.0 -> 23.2 us), and costs a little where
+// they are not (100,000 x 784 -> 1024: 489 -> 505 us).
+bool plan_two(const Shape& a, const Shape& b, Plan* qa, Plan* qb)
+{
+    *qa = plan_product(a);
+    *qb = plan_product(b);
+    if (plan_cycles(*qa, a) + plan_cycles(*qb, b) > 2e5) return false;
+    const Plan a2 = plan_product(a, 2), b2 = plan_product(b, 2), a1 = plan_product(a, 1), b1 = plan_product(b, 1);
+    const bool pairs = plan_cycles(a2, a) + plan_cycles(b2, b) <= plan_cycles(a1, a) + plan_cycles(b1, b);
+    *qa = pairs ? a2 : a1;
+    *qb = pairs ? b2 : b1;
+    return true;
 }
 
 // Opts a kernel in to `bytes` of dynamic shared memory, once per device.
@@ -368,22 +387,21 @@ knng_gpu_status allow_smem(uint32_t bytes)
     return KNNG_GPU_OK;
 }
 
-template <int CG, bool AMN, bool BMN, int EPI, bool LONG>
-knng_gpu_status launch_product_t(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const CUtensorMap& pre,
-                               const ProductParams& p, cudaStream_t st)
+template <int CG, int EPI, bool LONG, int N, int LAY>
+knng_gpu_status launch_product_t(const ProductCall<N>& call, cudaStream_t st)
 {
-    constexpr auto* kern = product_kernel<CG, AMN, BMN, EPI, LONG>;
+    constexpr auto* kern = product_kernel<CG, EPI, LONG, N, LAY>;
     // Units that fit the device at once (the same on every GPU this library is built for).
     static std::atomic<uint32_t> fit{0};
     uint32_t units = fit.load(std::memory_order_acquire);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[2];
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = CG;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.blockDim = dim3(pk_threads(CG, EPI, LONG));
     cfg.dynamicSmemBytes = kPkSmem;
     cfg.stream = st;
@@ -393,7 +411,7 @@ knng_gpu_status launch_product_t(const CUtensorMap& a, const CUtensorMap& b, con
     if (units == 0) {
         // The kernel's roles trade registers within what the launch gives them.
         constexpr int kWarps = pk_epi_warps(CG, EPI, LONG);
-        static_assert(4 * kPkIssueRegs + kWarps * pk_epi_regs(kWarps) <= (4 + kWarps) * pk_launch_regs(kWarps),
+        static_assert(4 * pk_issue_regs(kWarps) + kWarps * pk_epi_regs(kWarps) <= (4 + kWarps) * pk_launch_regs(kWarps),
                       "register split");
         cudaFuncAttributes fa;
         KNNG_CUDA(cudaFuncGetAttributes(&fa, kern));
@@ -408,36 +426,36 @@ knng_gpu_status launch_product_t(const CUtensorMap& a, const CUtensorMap& b, con
         }
         fit.store(units, std::memory_order_release);
     }
-    cfg.gridDim = dim3(std::min(units, p.items) * CG);
+    uint32_t items = call.p[0].items;
+    if (N == 2) items += call.p[N - 1].items;
+    cfg.gridDim = dim3(std::min(units, items) * CG);
     cfg.numAttrs = 2;
-    KNNG_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b, o, pre, p));
+    KNNG_CUDA(cudaLaunchKernelEx(&cfg, kern, call));
     return KNNG_GPU_OK;
 }
 
-template <int CG, bool AMN, bool BMN, int EPI>
-knng_gpu_status launch_product(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, const CUtensorMap& pre,
-                               const ProductParams& p, cudaStream_t st)
+template <int EPI, int N, int LAY>
+knng_gpu_status launch_product_l(int cg, const ProductCall<N>& call, cudaStream_t st)
 {
-    return p.pieces > p.splits ? launch_product_t<CG, AMN, BMN, EPI, true>(a, b, o, pre, p, st)
-                               : launch_product_t<CG, AMN, BMN, EPI, false>(a, b, o, pre, p, st);
+    bool longk = call.p[0].pieces > call.p[0].splits;
+    if (N == 2) longk = longk || call.p[N - 1].pieces > call.p[N - 1].splits;
+    if (cg == 2)
+        return longk ? launch_product_t<2, EPI, true, N, LAY>(call, st) : launch_product_t<2, EPI, false, N, LAY>(call, st);
+    return longk ? launch_product_t<1, EPI, true, N, LAY>(call, st) : launch_product_t<1, EPI, false, N, LAY>(call, st);
 }
 
-enum Layout { kKK = 0, kKMN = 1, kMNMN = 2 };  // how A and B are stored
-
-template <int EPI>
-knng_gpu_status launch_any(int cg, Layout lay, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o,
-                           const CUtensorMap& pre, const ProductParams& p, cudaStream_t st)
+template <int EPI, int N>
+knng_gpu_status launch_product(int cg, const ProductCall<N>& call, cudaStream_t st)
 {
-    if constexpr (EPI == kEpiStore) {
-        if (lay == kKMN)
-            return cg == 2 ? launch_product<2, false, true, EPI>(a, b, o, pre, p, st)
-                           : launch_product<1, false, true, EPI>(a, b, o, pre, p, st);
-        if (lay == kMNMN)
-            return cg == 2 ? launch_product<2, true, true, EPI>(a, b, o, pre, p, st)
-                           : launch_product<1, true, true, EPI>(a, b, o, pre, p, st);
+    if constexpr (N == 2) {
+        return launch_product_l<EPI, N, kAnyLayout>(cg, call, st);
+    } else {
+        if constexpr (EPI == kEpiStore) {
+            if (call.p[0].layout == kKMN) return launch_product_l<EPI, N, kKMN>(cg, call, st);
+            if (call.p[0].layout == kMNMN) return launch_product_l<EPI, N, kMNMN>(cg, call, st);
+        }
+        return launch_product_l<EPI, N, kKK>(cg, call, st);
     }
-    return cg == 2 ? launch_product<2, false, false, EPI>(a, b, o, pre, p, st)
-                   : launch_product<1, false, false, EPI>(a, b, o, pre, p, st);
 }
 
 knng_gpu_status operand_maps(const Plan& q, const Operand& a, const Operand& b, Layout lay, int in_type, CUtensorMap* ma,
@@ -449,7 +467,8 @@ knng_gpu_status operand_maps(const Plan& q, const Operand& a, const Operand& b, 
 
 int operand_type(int dtype) { return dtype == KNNG_DTYPE_F16 ? kF16 : kBF16; }
 
-ProductParams base_params(const Shape& s, const Plan& q, const Operand& a, const Operand& b, int dtype, int* err)
+ProductParams base_params(const Shape& s, const Plan& q, const Operand& a, const Operand& b, Layout lay, int dtype,
+                          int* err)
 {
     ProductParams p = {};
     p.m = static_cast<uint32_t>(s.m);
@@ -467,6 +486,7 @@ ProductParams base_params(const Shape& s, const Plan& q, const Operand& a, const
     p.plane_a = a.plane;
     p.plane_b = b.plane;
     p.in_type = operand_type(dtype);
+    p.layout = lay;
     p.error = err;
     p.wait_limit = kSpinLimitCycles;
     p.alpha = 1.0f;
@@ -490,21 +510,22 @@ struct Tail {
     uint32_t alpha_parts = 0;
 };
 
-// D = A B^T through the tail; where the plan splits K, the pieces in `part` and
-// the work of joining them in *join.
-knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, const Operand& b, Layout lay, int dtype,
-                              const Tail& t, float* part, JoinParams* join, int* err, cudaStream_t st)
+// Product i of a call: D = A B^T through the tail; where the plan splits K,
+// the pieces go to `part` and the work of joining them into *join.
+template <int N>
+knng_gpu_status set_store(ProductCall<N>& call, int i, const Shape& s, const Plan& q, const Operand& a, const Operand& b,
+                          Layout lay, int dtype, const Tail& t, float* part, JoinParams* join, int* err)
 {
-    CUtensorMap ma, mb, mo, mp;
-    KNNG_TRY(operand_maps(q, a, b, lay, operand_type(dtype), &ma, &mb));
-    ProductParams p = base_params(s, q, a, b, dtype, err);
+    KNNG_TRY(operand_maps(q, a, b, lay, operand_type(dtype), &call.map_a[i], &call.map_b[i]));
+    ProductParams& p = call.p[i];
+    p = base_params(s, q, a, b, lay, dtype, err);
+    call.map_out[i] = call.map_a[i];
+    call.map_pre[i] = call.map_a[i];
     if (q.splits > 1) {
         p.out = part;
         p.out_type = kF32;
         p.out_tma = 1;
         p.split_rows = static_cast<uint32_t>(q.split_rows);
-        KNNG_TRY(make_map(&mo, KNNG_DTYPE_F32, part, q.part_pitch, q.splits * q.split_rows, q.part_pitch, 32, 32));
-        KNNG_TRY(launch_any<kEpiStore>(q.cg, lay, ma, mb, mo, mo, p, st));
         JoinParams& j = *join;
         j.part = part;
         j.splits = q.splits;
@@ -526,7 +547,7 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
         j.pre = t.pre;
         j.ldp = t.ldp;
         j.blocks = join_blocks(s.m, s.n);
-        return KNNG_GPU_OK;
+        return make_map(&call.map_out[i], KNNG_DTYPE_F32, part, q.part_pitch, q.splits * q.split_rows, q.part_pitch, 32, 32);
     }
     p.out = t.out;
     p.ldo = t.ldo;
@@ -545,11 +566,9 @@ knng_gpu_status product_store(const Shape& s, const Plan& q, const Operand& a, c
     p.alpha = t.alpha;
     p.alpha_dev = t.alpha_dev;
     p.alpha_parts = t.alpha_parts;
-    mo = ma;
-    mp = ma;
-    if (p.out_tma) KNNG_TRY(make_map(&mo, t.out_type, t.out, s.n, s.m, t.ldo, 32, 32));
-    if (p.pre_tma) KNNG_TRY(make_map(&mp, t.aux_type, t.pre, s.n, s.m, t.ldp, 32, 32));
-    return launch_any<kEpiStore>(q.cg, lay, ma, mb, mo, mp, p, st);
+    if (p.out_tma) KNNG_TRY(make_map(&call.map_out[i], t.out_type, t.out, s.n, s.m, t.ldo, 32, 32));
+    if (p.pre_tma) KNNG_TRY(make_map(&call.map_pre[i], t.aux_type, t.pre, s.n, s.m, t.ldp, 32, 32));
+    return KNNG_GPU_OK;
 }
 
 // ------------------------------------------------------------------ checks
@@ -730,7 +749,9 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     t.aux_type = a.dtype;
     t.activation = a.activation;
     JoinParams join = {};
-    KNNG_TRY(product_store(s, q, operand(x, a.dtype, xs), operand(w, a.dtype, wst), kKK, a.dtype, t, part, &join, err, st));
+    ProductCall<1> call;
+    KNNG_TRY(set_store(call, 0, s, q, operand(x, a.dtype, xs), operand(w, a.dtype, wst), kKK, a.dtype, t, part, &join, err));
+    KNNG_TRY(launch_product<kEpiStore>(q.cg, call, st));
     return finish(SumsJob{}, join, JoinParams{}, st);
 }
 
@@ -779,7 +800,8 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
     // dz lies in the workspace unless it is dy and TMA can read that.
     const bool make_dz = products && (slope || needs_stage(dy, a.dtype));
     const Shape sx{a.m, a.k, a.n, combos, f32, a.dtype == KNNG_DTYPE_BF16}, sw{a.n, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16};
-    const Plan qx = plan_product(sx), qw = plan_product(sw);
+    Plan qx = plan_product(sx), qw = plan_product(sw);
+    const bool merged = a.dx && a.dw && plan_two(sx, sw, &qx, &qw);
     KNNG_TRY(check_items(op, qx));
     KNNG_TRY(check_items(op, qw));
     const uint64_t pitch = stage_pitch(a.n, a.dtype);
@@ -834,12 +856,24 @@ knng_gpu_status linear_backward_run(const knng_gpu_linear_backward_args& a, void
                                          static_cast<uint32_t>(pitch)}
                                : operand(dy, a.dtype, nullptr);
     JoinParams join_x = {}, join_w = {};
-    if (a.dx)
-        KNNG_TRY(product_store(sx, qx, oz, operand(w, a.dtype, wst), kKMN, a.dtype, Tail{a.dx, a.k, a.dtype}, xpart, &join_x,
-                               err, st));
-    if (a.dw)
-        KNNG_TRY(product_store(sw, qw, oz, operand(x, a.dtype, xs), kMNMN, a.dtype, Tail{a.dw, a.k, a.dtype}, wpart,
-                               &join_w, err, st));
+    const Operand ow = operand(w, a.dtype, wst), ox = operand(x, a.dtype, xs);
+    const Tail tx{a.dx, a.k, a.dtype}, tw{a.dw, a.k, a.dtype};
+    if (merged) {
+        ProductCall<2> call;
+        KNNG_TRY(set_store(call, 0, sx, qx, oz, ow, kKMN, a.dtype, tx, xpart, &join_x, err));
+        KNNG_TRY(set_store(call, 1, sw, qw, oz, ox, kMNMN, a.dtype, tw, wpart, &join_w, err));
+        KNNG_TRY(launch_product<kEpiStore>(qx.cg, call, st));
+    } else {
+        ProductCall<1> call;
+        if (a.dx) {
+            KNNG_TRY(set_store(call, 0, sx, qx, oz, ow, kKMN, a.dtype, tx, xpart, &join_x, err));
+            KNNG_TRY(launch_product<kEpiStore>(qx.cg, call, st));
+        }
+        if (a.dw) {
+            KNNG_TRY(set_store(call, 0, sw, qw, oz, ox, kMNMN, a.dtype, tw, wpart, &join_w, err));
+            KNNG_TRY(launch_product<kEpiStore>(qw.cg, call, st));
+        }
+    }
     return finish(db, join_x, join_w, st);
 }
 
@@ -919,9 +953,11 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
         KNNG_TRY(take_error(&err));
         KNNG_TRY(prepare(a.dtype, stage_job(x, a.dtype, xs), stage_job(w, a.dtype, wst), GradRowsJob{}, st));
         const Operand ox = operand(x, a.dtype, xs), ow = operand(w, a.dtype, wst);
-        CUtensorMap ma, mb;
-        KNNG_TRY(operand_maps(q, ox, ow, kKK, operand_type(a.dtype), &ma, &mb));
-        ProductParams p = base_params(s, q, ox, ow, a.dtype, err);
+        ProductCall<1> call;
+        KNNG_TRY(operand_maps(q, ox, ow, kKK, operand_type(a.dtype), &call.map_a[0], &call.map_b[0]));
+        call.map_out[0] = call.map_pre[0] = call.map_a[0];
+        ProductParams& p = call.p[0];
+        p = base_params(s, q, ox, ow, kKK, a.dtype, err);
         p.segments = segments;
         p.items = q.tiles_m * segments;
         p.scale2 = scale2;
@@ -930,7 +966,7 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
         p.classes = static_cast<uint32_t>(a.n);
         p.part = part;
         p.label_dot = label_dot;
-        KNNG_TRY(launch_any<kEpiSoftmax>(q.cg, kKK, ma, mb, ma, ma, p, st));
+        KNNG_TRY(launch_product<kEpiSoftmax>(q.cg, call, st));
     }
     // A block per row where there are few rows with many pieces, a warp per row otherwise.
     if (pieces > 64 && a.m < sm_count() * 8)
@@ -948,6 +984,7 @@ constexpr uint64_t kPieceBytes = 256ull << 20;
 struct GradPlan {
     uint64_t width;      // columns of a piece, the last one narrower
     Plan g, dx, dw, dw_last;
+    bool merged;         // dx and dw in one launch
 };
 
 Plan plan_grad_tiles(const Shape& s)
@@ -974,9 +1011,8 @@ GradPlan plan_grad(uint64_t m, uint64_t k, uint64_t n, int dtype)
         const Shape sg{m, p.width, k, combos, f32, bf16}, sx{m, k, p.width, combos, f32, bf16};
         const Shape sw{p.width, k, m, combos, f32, bf16}, sl{n - (count - 1) * p.width, k, m, combos, f32, bf16};
         p.g = plan_grad_tiles(sg);
-        p.dx = plan_product(sx);
-        p.dw = plan_product(sw);
-        p.dw_last = count > 1 ? plan_product(sl) : p.dw;
+        p.merged = plan_two(sx, sw, &p.dx, &p.dw);
+        p.dw_last = count > 1 ? plan_product(sl, p.merged ? p.dx.cg : 0) : p.dw;
         const double c = static_cast<double>(count) * (plan_cycles(p.g, sg) + plan_cycles(p.dx, sx) + plan_cycles(p.dw, sw));
         if (least == 0.0 || c < least) {
             least = c;
@@ -1052,9 +1088,10 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         const Shape s1{a.m, cols, a.k, combos, f32, a.dtype == KNNG_DTYPE_BF16};
         const bool last = c0 + width >= a.n;
         const Plan q1 = last ? plan_grad_tiles(s1) : plan.g;
-        CUtensorMap ma, mb, mo;
-        KNNG_TRY(operand_maps(q1, ox, wp, kKK, operand_type(a.dtype), &ma, &mb));
-        ProductParams p = base_params(s1, q1, ox, wp, a.dtype, err);
+        ProductCall<1> call;
+        KNNG_TRY(operand_maps(q1, ox, wp, kKK, operand_type(a.dtype), &call.map_a[0], &call.map_b[0]));
+        ProductParams& p = call.p[0];
+        p = base_params(s1, q1, ox, wp, kKK, a.dtype, err);
         p.scale2 = a.scale * 1.44269504088896f;
         p.labels = a.labels;
         p.labels_i64 = a.labels_i64;
@@ -1070,9 +1107,41 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
         p.grad_pitch = static_cast<uint32_t>(gpitch);
         const uint64_t gld = gpitch * planes;
         const uint64_t gwidth = planes == 1 ? cols : gld;
-        KNNG_TRY(make_map(&mo, operand_type(a.dtype), g, gwidth, a.m, gld, 32, 32));
-        KNNG_TRY(launch_any<kEpiGrad>(q1.cg, kKK, ma, mb, mo, mo, p, st));
+        KNNG_TRY(make_map(&call.map_out[0], operand_type(a.dtype), g, gwidth, a.m, gld, 32, 32));
+        call.map_pre[0] = call.map_out[0];
+        KNNG_TRY(launch_product<kEpiGrad>(q1.cg, call, st));
         const Operand og{g, a.m, gwidth, gld, static_cast<uint32_t>(gpitch)};
+        ProductCall<2> both;  // dx first: its items are the longer ones
+        ProductCall<1> one;
+        const bool merged = plan.merged && a.dx && a.dw;
+        if (a.dx) {
+            // Pieces add up in fp32, scaled when they are joined: the first one stores, the others add.
+            const Shape sp{a.m, a.k, cols, combos, f32, a.dtype == KNNG_DTYPE_BF16};
+            Plan qp = qx;
+            qp.kblocks = static_cast<uint32_t>(ceil_div(cols, 64));
+            qp.splits = std::min(qx.splits, qp.pieces());
+            ProductParams px = base_params(sp, qp, og, wp, kKMN, a.dtype, err);
+            px.out = xpart;
+            px.out_type = kF32;
+            px.out_tma = 1;
+            px.accumulate = c0 > 0;
+            px.split_rows = static_cast<uint32_t>(xpart_rows);
+            CUtensorMap mga, mwb, mx;
+            KNNG_TRY(operand_maps(qp, og, wp, kKMN, operand_type(a.dtype), &mga, &mwb));
+            KNNG_TRY(make_map(&mx, KNNG_DTYPE_F32, xpart, xpart_pitch, qx.splits * xpart_rows, xpart_pitch, 32, 32));
+            const auto set = [&](auto& call) {
+                call.map_a[0] = mga;
+                call.map_b[0] = mwb;
+                call.map_out[0] = call.map_pre[0] = mx;
+                call.p[0] = px;
+            };
+            if (merged) {
+                set(both);
+            } else {
+                set(one);
+                KNNG_TRY(launch_product<kEpiStore>(qp.cg, one, st));
+            }
+        }
         if (a.dw) {
             const Shape sw{cols, a.k, a.m, combos, f32, a.dtype == KNNG_DTYPE_BF16};
             const Plan& qw = last && c0 > 0 ? plan.dw_last : plan.dw;
@@ -1080,27 +1149,16 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
             t.alpha = 1.0f / gscale;
             t.alpha_dev = cmax;
             t.alpha_parts = row_blocks;
-            KNNG_TRY(product_store(sw, qw, og, ox, kMNMN, a.dtype, t, wpart, &join_w, err, st));
-            // The last piece's joins wait for dx.
-            if (!last) KNNG_TRY(finish(SumsJob{}, join_w, JoinParams{}, st));
+            if (merged) {
+                KNNG_TRY(set_store(both, 1, sw, qw, og, ox, kMNMN, a.dtype, t, wpart, &join_w, err));
+                KNNG_TRY(launch_product<kEpiStore>(qw.cg, both, st));
+            } else {
+                KNNG_TRY(set_store(one, 0, sw, qw, og, ox, kMNMN, a.dtype, t, wpart, &join_w, err));
+                KNNG_TRY(launch_product<kEpiStore>(qw.cg, one, st));
+            }
         }
-        if (a.dx) {
-            // Pieces add up in fp32: the first one stores, the others add.
-            const Shape sp{a.m, a.k, cols, combos, f32, a.dtype == KNNG_DTYPE_BF16};
-            Plan qp = qx;
-            qp.kblocks = static_cast<uint32_t>(ceil_div(cols, 64));
-            qp.splits = std::min(qx.splits, qp.pieces());
-            CUtensorMap mga, mwb, mx;
-            KNNG_TRY(operand_maps(qp, og, wp, kKMN, operand_type(a.dtype), &mga, &mwb));
-            ProductParams px = base_params(sp, qp, og, wp, a.dtype, err);
-            px.out = xpart;
-            px.out_type = kF32;
-            px.out_tma = 1;
-            px.accumulate = c0 > 0;
-            px.split_rows = static_cast<uint32_t>(xpart_rows);
-            KNNG_TRY(make_map(&mx, KNNG_DTYPE_F32, xpart, xpart_pitch, qx.splits * xpart_rows, xpart_pitch, 32, 32));
-            KNNG_TRY(launch_any<kEpiStore>(qp.cg, kKMN, mga, mwb, mx, mx, px, st));
-        }
+        // The last piece's joins wait for dx's.
+        if (!last) KNNG_TRY(finish(SumsJob{}, join_w, JoinParams{}, st));
     }
     JoinParams j = {};
     if (a.dx) {

@@ -47,6 +47,7 @@ constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkBoxes + 512 + 1024;
 
 enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+enum Layout : int { kKK = 0, kKMN = 1, kMNMN = 2, kAnyLayout = 3 };  // how A and B are stored
 enum Epilogue : int { kEpiStore = 0, kEpiSoftmax = 1, kEpiGrad = 2 };
 
 struct ProductParams {
@@ -62,6 +63,7 @@ struct ProductParams {
     uint32_t planes;               // 1, or 3 parts of split fp32 operands
     uint32_t plane_a, plane_b;     // columns from one plane to the next in the stored matrices
     int in_type;                   // kBF16 or kF16
+    int layout;                    // Layout of A and B
     int* error;
     long long wait_limit;
     // store
@@ -77,8 +79,8 @@ struct ProductParams {
     int aux_type;
     int bias_vec, residual_vec;    // they allow 16-byte loads
     int activation;
-    float alpha;                   // D is scaled by alpha * *alpha_dev
-    const float* alpha_dev;        // the largest of alpha_parts values
+    float alpha;                   // D is scaled by alpha and, the last product of a call, by
+    const float* alpha_dev;        // the largest of alpha_parts values there
     uint32_t alpha_parts;
     // softmax and gradient
     float scale2;                  // scale * log2(e)
@@ -93,6 +95,13 @@ struct ProductParams {
     float grad_scale;              // gradient: power of two on the stored values
     uint32_t grad_planes, grad_pitch;
     float* label_rest;             // gradient: what rounding took from the label's entry (one plane)
+};
+
+// N products in one launch, the items of the second after those of the first.
+template <int N>
+struct ProductCall {
+    CUtensorMap map_a[N], map_b[N], map_out[N], map_pre[N];
+    ProductParams p[N];
 };
 
 // ---------------------------------------------------------------- PTX of this kernel
@@ -459,17 +468,20 @@ __host__ __device__ constexpr int pk_epi_warps(int cg, int epi, bool longk)
 __host__ __device__ constexpr int pk_threads(int cg, int epi, bool longk) { return 128 + 32 * pk_epi_warps(cg, epi, longk); }
 // Registers a thread: what the launch gives, and the split after setmaxnreg
 // between the first warpgroup and those of the epilogue. The split never sums
-// to more than the launch gave: 56 + 2 * 224 = 3 * 168, 56 + 4 * 104 < 5 * 96.
+// to more than the launch gave: 72 + 2 * 216 = 3 * 168, 64 + 4 * 104 = 5 * 96.
 __host__ __device__ constexpr int pk_launch_regs(int warps) { return warps == 8 ? 168 : 96; }
-constexpr int kPkIssueRegs = 56;
-__host__ __device__ constexpr int pk_epi_regs(int warps) { return warps == 8 ? 224 : 104; }
+__host__ __device__ constexpr int pk_issue_regs(int warps) { return warps == 8 ? 72 : 64; }
+__host__ __device__ constexpr int pk_epi_regs(int warps) { return warps == 8 ? 216 : 104; }
 
 // LONG: an item may have several K pieces, whose sums are added in registers.
-template <int CG, bool AMN, bool BMN, int EPI, bool LONG>
+// N = 2: the two products of a backward pass, which need only part of the GPU
+// each when they are small and an uneven last round when they are not; plain
+// stores.
+// LAY: how the operands lie, or kAnyLayout to take it from each product (known
+// at compile time it saves the issuing threads 5 to 10 % of a long product).
+template <int CG, int EPI, bool LONG, int N, int LAY>
 __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
-                   const ProductParams p)
+    product_kernel(const __grid_constant__ ProductCall<N> call)
 {
     constexpr int EW = pk_epi_warps(CG, EPI, LONG);
     // Softmax with 16 warps: eight for each of the two accumulator buffers, so
@@ -480,8 +492,9 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
     constexpr int kGroups = EW / 4 / kSets;  // warps that share a quarter of the rows of a tile
     constexpr uint32_t kBufCols = 128 * CG;  // TMEM columns of an accumulator buffer
     constexpr uint32_t kTmemCols = 2 * kBufCols;
-    const uint32_t bn_tile = p.tile_n;
-    const uint32_t bn_cta = bn_tile / CG;    // rows of B that this CTA stages
+    const uint32_t items0 = call.p[0].items;
+    const uint32_t items = items0 + (N == 2 ? call.p[N - 1].items : 0u);
+    const long long wait_limit = call.p[0].wait_limit;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stage_base = smem;
@@ -512,8 +525,10 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         }
         *abort_flag = 0;
         fence_barrier_init();
-        prefetch_tensormap(&map_a);
-        prefetch_tensormap(&map_b);
+        for (int i = 0; i < N; ++i) {
+            prefetch_tensormap(&call.map_a[i]);
+            prefetch_tensormap(&call.map_b[i]);
+        }
     }
     if (warp == 1) {
         if constexpr (CG == 2)
@@ -531,7 +546,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
     previous_done();
 
     auto abort_all = [&]() {
-        *p.error = 1;
+        *call.p[0].error = 1;
         __threadfence_system();
         *abort_flag = 1;
         if constexpr (CG == 2) st_cluster_u32(mapa_shared(smem_u32(const_cast<int*>(abort_flag)), cta ^ 1u), 1u);
@@ -539,30 +554,38 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pk_issue_regs(EW)));
         if (lane == 0) {
             const uint32_t full_leader = CG == 2 ? mapa_shared(smem_u32(full), 0u) : 0u;
-            const uint32_t b_bytes = BMN ? (bn_cta > 64 ? 16384u : 8192u) : bn_cta * 128u;
-            const uint32_t tx = CG * (kPkStageBytes / 2 + b_bytes);
             uint32_t stage = 0, phase = 0, issued = 0;
             bool ok = true;
-            for (uint32_t i = unit; ok && i < p.items; i += units) {
-                const Item t = decode_item<EPI>(p, i);
+            for (uint32_t i = unit; ok && i < items; i += units) {
+                const int which = N == 2 && i >= items0;
+                const ProductParams& p = call.p[which];
+                const CUtensorMap* map_a = &call.map_a[which];
+                const CUtensorMap* map_b = &call.map_b[which];
+                const int lay = LAY == kAnyLayout ? p.layout : LAY;
+                const bool a_mn = lay == kMNMN, b_mn = lay != kKK;
+                const uint32_t bn_tile = p.tile_n, bn_cta = bn_tile / CG;  // rows of B that this CTA stages
+                const uint32_t b_bytes = b_mn ? (bn_cta > 64 ? 16384u : 8192u) : bn_cta * 128u;
+                const uint32_t tx = CG * (kPkStageBytes / 2 + b_bytes);
+                const uint32_t planes = p.planes, plane_a = p.plane_a, plane_b = p.plane_b;
+                const Item t = decode_item<EPI>(p, which ? i - items0 : i);
                 const int32_t am = static_cast<int32_t>(t.tm * (128 * CG) + cta * 128);
                 for (uint32_t tn = t.n0; ok && tn < t.n1; ++tn) {
                     const int32_t bn = static_cast<int32_t>(tn * bn_tile + cta * bn_cta);
                     const uint32_t kb1 = min(t.p1 * p.piece, p.kblocks);
-                    uint32_t kb = t.p0 * p.piece, plane = p.planes;
+                    uint32_t kb = t.p0 * p.piece, plane = planes;
                     while (kb < kb1) {
                         const int32_t k = static_cast<int32_t>(kb * 64);
                         --plane;  // the smallest plane of a K block first
-                        const int32_t pa = static_cast<int32_t>(plane * p.plane_a);
-                        const int32_t pb = static_cast<int32_t>(plane * p.plane_b);
+                        const int32_t pa = static_cast<int32_t>(plane * plane_a);
+                        const int32_t pb = static_cast<int32_t>(plane * plane_b);
                         if (plane == 0) {
-                            plane = p.planes;
+                            plane = planes;
                             ++kb;
                         }
-                        ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.wait_limit);
+                        ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, wait_limit);
                         if (!ok) break;
                         uint8_t* sa = stage_base + stage * kPkStageBytes;
                         uint8_t* sb = sa + kPkStageBytes / 2;
@@ -573,17 +596,17 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                             else
                                 tma_load_2d(dst, map, x, y, &full[stage]);
                         };
-                        if constexpr (AMN) {
-                            load(sa, &map_a, pa + am, k);
-                            load(sa + 8192, &map_a, pa + am + 64, k);
+                        if (a_mn) {
+                            load(sa, map_a, pa + am, k);
+                            load(sa + 8192, map_a, pa + am + 64, k);
                         } else {
-                            load(sa, &map_a, pa + k, am);
+                            load(sa, map_a, pa + k, am);
                         }
-                        if constexpr (BMN) {
-                            load(sb, &map_b, pb + bn, k);
-                            if (bn_cta > 64) load(sb + 8192, &map_b, pb + bn + 64, k);
+                        if (b_mn) {
+                            load(sb, map_b, pb + bn, k);
+                            if (bn_cta > 64) load(sb + 8192, map_b, pb + bn + 64, k);
                         } else {
-                            load(sb, &map_b, pb + k, bn);
+                            load(sb, map_b, pb + k, bn);
                         }
                         ++issued;
                         if (++stage == kPkStages) {
@@ -601,7 +624,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                     for (uint32_t s = 0; s < kPkStages; ++s) {
                         if (issued <= s) break;
                         const uint32_t uses = (issued - s - 1) / kPkStages;  // 0-based index of its last use
-                        (void)mbar_wait_drain(&full[s], uses & 1, p.wait_limit / 8);
+                        (void)mbar_wait_drain(&full[s], uses & 1, wait_limit / 8);
                     }
                 }
             }
@@ -609,32 +632,37 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------ UMMA issuer
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pk_issue_regs(EW)));
         if (leader && lane == 0) {
-            const uint32_t fmt = p.in_type == kBF16 ? 1u : 0u;
-            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (AMN ? 1u << 15 : 0u) |
-                                   (BMN ? 1u << 16 : 0u) | ((bn_tile >> 3) << 17) |
-                                   (static_cast<uint32_t>((128 * CG) >> 4) << 24);
             const uint32_t s0 = smem_u32(stage_base);
-            const uint64_t a0 = AMN ? umma_desc_mn_sw128(s0) : umma_desc_sw128(s0);
-            const uint64_t b0 = BMN ? umma_desc_mn_sw128(s0 + kPkStageBytes / 2) : umma_desc_sw128(s0 + kPkStageBytes / 2);
-            constexpr uint64_t ka = AMN ? 2048 >> 4 : 2;  // 16 of K: 16 rows of 128 bytes, or 32 bytes
-            constexpr uint64_t kb = BMN ? 2048 >> 4 : 2;
             uint32_t stage = 0, phase = 0, acc = 0;
             bool ok = true;
-            for (uint32_t i = unit; ok && i < p.items; i += units) {
-                const Item t = decode_item<EPI>(p, i);
+            for (uint32_t i = unit; ok && i < items; i += units) {
+                const int which = N == 2 && i >= items0;
+                const ProductParams& p = call.p[which];
+                const int lay = LAY == kAnyLayout ? p.layout : LAY;
+                const bool a_mn = lay == kMNMN, b_mn = lay != kKK;
+                const uint32_t fmt = p.in_type == kBF16 ? 1u : 0u;
+                const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn ? 1u << 15 : 0u) |
+                                       (b_mn ? 1u << 16 : 0u) | ((p.tile_n >> 3) << 17) |
+                                       (static_cast<uint32_t>((128 * CG) >> 4) << 24);
+                const uint64_t a0 = a_mn ? umma_desc_mn_sw128(s0) : umma_desc_sw128(s0);
+                const uint64_t b0 = b_mn ? umma_desc_mn_sw128(s0 + kPkStageBytes / 2) : umma_desc_sw128(s0 + kPkStageBytes / 2);
+                const uint64_t ka = a_mn ? 2048 >> 4 : 2;  // 16 of K: 16 rows of 128 bytes, or 32 bytes
+                const uint64_t kb = b_mn ? 2048 >> 4 : 2;
+                const uint32_t planes = p.planes;
+                const Item t = decode_item<EPI>(p, which ? i - items0 : i);
                 const uint32_t pieces = (t.n1 - t.n0) * (t.p1 - t.p0);
                 for (uint32_t q = 0; ok && q < pieces; ++q, ++acc) {
                     const uint32_t piece = t.p0 + q % (t.p1 - t.p0);
                     const uint32_t blocks = min((piece + 1) * p.piece, p.kblocks) - piece * p.piece;
                     const uint32_t buf = acc & 1u;
-                    ok = mbar_wait_sleep(&tempty[buf], ((acc >> 1) & 1u) ^ 1u, abort_flag, p.wait_limit);
+                    ok = mbar_wait_sleep(&tempty[buf], ((acc >> 1) & 1u) ^ 1u, abort_flag, wait_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem_base + buf * kBufCols;
                     auto stage_ready = [&]() {
-                        const bool r = mbar_wait_sleep(&full[stage], phase, abort_flag, p.wait_limit);
+                        const bool r = mbar_wait_sleep(&full[stage], phase, abort_flag, wait_limit);
                         tc_fence_after();
                         return r;
                     };
@@ -663,7 +691,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         else
                             umma_commit(&empty[s]);
                     };
-                    if (p.planes == 1) {
+                    if (planes == 1) {
                         for (uint32_t kk = 0; kk < blocks; ++kk) {
                             ok = stage_ready();
                             if (!ok) break;
@@ -716,7 +744,8 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         // 32-column chunks of this warp: number group, group + kGroups, ...
         constexpr int kMaxChunks = 4 * CG / kGroups;
         constexpr uint32_t kStep = 32 * kGroups;  // columns from one to the next
-        const int chunks = static_cast<int>((bn_tile / 32 + kGroups - 1 - group) / kGroups);
+        int chunks = 0;  // of the current item
+        const ProductParams* at_work = &call.p[0];  // the current item's product
         constexpr int kBox = kPkBoxes / EW / 2;
         uint8_t* box = boxes + e * 2 * kBox;
         uint32_t nbox = 0;  // boxes sent: picks the buffer
@@ -769,6 +798,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         };
         // Element stores of a box to rows that TMA cannot write.
         auto copy_out = [&](const uint8_t* b, void* dst, uint64_t ld, int esize, uint32_t row0, uint32_t col0) {
+            const ProductParams& p = *at_work;
             __syncwarp();
             const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
             if (col0 + lane < p.n) {
@@ -801,7 +831,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         };
         auto wait_acc = [&](uint32_t& buf) -> bool {
             buf = acc & 1u;
-            if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, p.wait_limit)) return false;
+            if (!mbar_wait(&tfull[buf], (acc >> 1) & 1u, abort_flag, wait_limit)) return false;
             ++acc;
             tc_fence_after();
             return true;
@@ -865,15 +895,23 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
             return true;
         };
 
-        const float largest = p.alpha_dev ? warp_largest(p.alpha_dev, p.alpha_parts) : 1.0f;
-        for (uint32_t it = unit; ok && it < p.items; it += units) {
-            const Item t = decode_item<EPI>(p, it);
+        // Only the last product of a call is scaled by it.
+        const ProductParams& scaled = call.p[N - 1];
+        const float largest = scaled.alpha_dev ? warp_largest(scaled.alpha_dev, scaled.alpha_parts) : 1.0f;
+        for (uint32_t it = unit; ok && it < items; it += units) {
+            const int which = N == 2 && it >= items0;
+            if constexpr (N == 2) at_work = &call.p[which];
+            const ProductParams& p = call.p[which];
+            const CUtensorMap* map_out = &call.map_out[which];
+            const uint32_t bn_tile = p.tile_n;
+            chunks = static_cast<int>((bn_tile / 32 + kGroups - 1 - group) / kGroups);
+            const Item t = decode_item<EPI>(p, which ? it - items0 : it);
             const uint32_t row0 = t.tm * (128 * CG) + cta * 128 + quarter * 32;
             const uint32_t row = row0 + lane;
             const bool live = row < p.m;
 
             if constexpr (EPI == kEpiStore) {
-                const float alpha = p.alpha * largest;
+                const float alpha = which == N - 1 ? p.alpha * largest : p.alpha;
                 const uint32_t col_base = t.n0 * bn_tile + group * 32;
                 const uint32_t out_row0 = row0 + t.split * p.split_rows;
                 ok = for_tile(t.p1 - t.p0, [&](float* v, int i) {
@@ -883,7 +921,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] *= alpha;
                     }
-                    if (p.bias) {
+                    if (N == 1 && p.bias) {
                         if (p.bias_vec && col + 32 <= p.n) {
                             if (p.aux_type == kF32) {
                                 const float4* q4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col);
@@ -905,7 +943,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                                 if (col + j < p.n) v[j] += load_elem(p.bias, col + j, p.aux_type);
                         }
                     }
-                    if (p.pre) {
+                    if (N == 1 && p.pre) {
                         // The value before the activation, rounded to the inputs' type.
                         uint8_t* b = next_box(p.aux_type == kF32);
                         if (p.aux_type == kF32) {
@@ -916,18 +954,18 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                             put_words(b, w);
                         }
                         if (p.pre_tma)
-                            send(b, &map_pre, col, row0, false);
+                            send(b, &call.map_pre[0], col, row0, false);
                         else
                             copy_out(b, p.pre, p.ldp, p.aux_type == kF32 ? 4 : 2, row0, col);
                     }
-                    switch (p.activation) {
+                    switch (N == 1 ? p.activation : 0) {
                         case kActRelu: act_all<kActRelu>(v); break;
                         case kActGelu: act_all<kActGelu>(v); break;
                         case kActGeluTanh: act_all<kActGeluTanh>(v); break;
                         case kActSilu: act_all<kActSilu>(v); break;
                         default: break;
                     }
-                    if (p.residual && live) {
+                    if (N == 1 && p.residual && live) {
                         const uint64_t at = row * p.ldr + col;
                         if (p.residual_vec && col + 32 <= p.n) {
                             if (p.aux_type == kF32) {
@@ -959,7 +997,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         put_words(b, w);
                     }
                     if (p.out_tma)
-                        send(b, &map_out, col, out_row0, p.accumulate != 0);
+                        send(b, map_out, col, out_row0, p.accumulate != 0);
                     else
                         copy_out(b, p.out, p.ldo, p.out_type == kF32 ? 4 : 2, row0, col);
                 });
@@ -1091,7 +1129,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                     pack32(v, w, p.in_type);
                     uint8_t* b = next_box();
                     put_words(b, w);
-                    send(b, &map_out, col, row0, false);
+                    send(b, map_out, col, row0, false);
                     if (p.grad_planes == 3) {
 #pragma unroll
                         for (int plane = 1; plane < 3; ++plane) {
@@ -1104,7 +1142,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                             pack32(v, w, kBF16);
                             b = next_box();
                             put_words(b, w);
-                            send(b, &map_out, plane * p.grad_pitch + col, row0, false);
+                            send(b, map_out, plane * p.grad_pitch + col, row0, false);
                         }
                     }
                 });
@@ -1114,7 +1152,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         if (lane == 0) bulk_wait_all();
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkIssueRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pk_issue_regs(EW)));
     }
 
     tc_fence_before();
