@@ -392,6 +392,10 @@ knng_gpu_status knng_gpu_softmax_xent_backward(const knng_gpu_softmax_xent_backw
  * reference, whose code has no device waits. */
 knng_gpu_status knng_gpu_selftest_bounded_wait(uint64_t wait_limit_cycles);
 
+/* The same for the product kernel of the calls on device rows, with CTA pairs
+ * and with single CTAs: KNNG_GPU_TIMEOUT when both unwind. */
+knng_gpu_status knng_gpu_selftest_product_wait(uint64_t wait_limit_cycles);
+
 #ifdef __cplusplus
 }
 #endif

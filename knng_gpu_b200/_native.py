@@ -56,6 +56,7 @@ GPU_SYMBOLS = (
     "knng_gpu_softmax_xent",
     "knng_gpu_softmax_xent_backward_workspace_bytes",
     "knng_gpu_softmax_xent_backward",
+    "knng_gpu_selftest_product_wait",
 )
 
 
@@ -156,6 +157,7 @@ def gpu_lib() -> ctypes.CDLL:
             "knng_gpu_pack_u8": (c_int, [c_void_p, c_uint64, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p]),
             "knng_gpu_knn_scratch_bytes": (c_uint64, [c_uint64, c_uint64]),
             "knng_gpu_selftest_bounded_wait": (c_int, [c_uint64]),
+            "knng_gpu_selftest_product_wait": (c_int, [c_uint64]),
             "knng_gpu_nccl_id_bytes": (c_uint64, []),
             "knng_gpu_nccl_unique_id": (c_int, [c_void_p]),
             "knng_gpu_comm_create": (c_int, [c_void_p, c_int, c_int, POINTER(c_void_p)]),

@@ -1189,6 +1189,31 @@ knng_gpu_status softmax_xent_backward_run(const knng_gpu_softmax_xent_backward_a
     return finish(SumsJob{}, join_w, j, st);
 }
 
+// ------------------------------------------------------------------ timeout test
+knng_gpu_status selftest_product(int cg, uint64_t limit)
+{
+    struct Buffer {
+        void* p = nullptr;
+        ~Buffer() { cudaFree(p); }
+    } rows, out;
+    constexpr uint64_t kRows = 256, kWidth = 128;
+    KNNG_CUDA(cudaMalloc(&rows.p, kRows * kWidth * 2));
+    KNNG_CUDA(cudaMalloc(&out.p, kRows * kRows * 2));
+    KNNG_CUDA(cudaMemset(rows.p, 0, kRows * kWidth * 2));
+    int* err;
+    KNNG_TRY(take_error(&err));
+    const Shape s{kRows, kRows, kWidth, 1, false, true};
+    const Operand a{rows.p, kRows, kWidth, kWidth, 0};
+    ProductCall<1> call;
+    KNNG_TRY(set_store(call, 0, s, tiles_of(s, cg, 128 * cg), a, a, kKK, KNNG_DTYPE_BF16,
+                       Tail{out.p, kRows, KNNG_DTYPE_BF16}, nullptr, nullptr, err));
+    call.p[0].wait_limit = static_cast<long long>(limit);
+    call.p[0].test_mode = 1;
+    KNNG_TRY(launch_product<kEpiStore>(cg, call, nullptr));
+    KNNG_CUDA(cudaStreamSynchronize(nullptr));
+    return take_error(&err);
+}
+
 // No exception leaves a C entry point.
 template <class F>
 knng_gpu_status guarded(F&& f)
@@ -1228,5 +1253,13 @@ KNNG_LEARN_ENTRY(linear)
 KNNG_LEARN_ENTRY(linear_backward)
 KNNG_LEARN_ENTRY(softmax_xent)
 KNNG_LEARN_ENTRY(softmax_xent_backward)
+
+knng_gpu_status knng_gpu_selftest_product_wait(uint64_t wait_limit_cycles)
+{
+    return guarded([&]() -> knng_gpu_status {
+        const knng_gpu_status pair = selftest_product(2, wait_limit_cycles);
+        return pair == KNNG_GPU_TIMEOUT ? selftest_product(1, wait_limit_cycles) : pair;
+    });
+}
 
 }  // extern "C"

@@ -66,6 +66,7 @@ struct ProductParams {
     int layout;                    // Layout of A and B
     int* error;
     long long wait_limit;
+    int test_mode;                 // 1: the producer withholds its first arrival (timeout test)
     // store
     int out_type;                  // ElemType
     int out_tma, pre_tma;          // TMA store possible; otherwise element stores through out / pre
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         if (!ok) break;
                         uint8_t* sa = stage_base + stage * kPkStageBytes;
                         uint8_t* sb = sa + kPkStageBytes / 2;
-                        if (leader) mbar_arrive_expect_tx(&full[stage], tx);
+                        if (leader && !(call.p[0].test_mode == 1 && issued == 0)) mbar_arrive_expect_tx(&full[stage], tx);
                         auto load = [&](uint8_t* dst, const CUtensorMap* map, int32_t x, int32_t y) {
                             if constexpr (CG == 2)
                                 tma_load_2d_pair(dst, map, x, y, full_leader + stage * 8);

@@ -386,3 +386,16 @@ def test_refusals_on_the_gpu(cuda_ok):
         with pytest.raises(kg.InvalidArgument):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_withheld_arrival_times_out_and_results_stay_right(cuda_ok):
+    # A wait of ~10 ms runs out, every role unwinds, the status says so once, and the context goes on.
+    from knng_gpu_b200 import _native
+
+    lib = _native.gpu_lib()
+    assert lib.knng_gpu_selftest_product_wait(20_000_000) == 3
+    assert b"bounded device wait" in lib.knng_gpu_last_error()
+    g = make_gen(60)
+    for m in (100, 3000):
+        x, w = rows(g, m, 256, BF16), rows(g, 512, 256, BF16)
+        check(kg.linear(x, w), *linear64(x, w, None, None, "none", BF16)[0], "out")
