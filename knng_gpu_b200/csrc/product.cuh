@@ -19,7 +19,7 @@
 // rows of B per 64-wide K block, half of what two single-CTA tiles would read
 // from L2. CG = 1: up to 128 x 128 by one CTA, for products with too few tiles to fill the
 // GPU with pairs. Per CTA:
-//   warp 0      TMA producer, kStages-deep ring of 32 KiB stages
+//   warp 0      TMA producer: as many stages as fit, 5 to 8
 //   warp 1      TMEM allocation; UMMA issue (leader CTA, one lane)
 //   warps 2-3   idle
 //   warps 4 on  epilogue (8 or 16 warps): thread = one accumulator row, the
@@ -40,10 +40,12 @@
 
 namespace knng_b200 {
 
-constexpr int kPkStages = 5;
-constexpr int kPkStageBytes = 32768;  // 128 x 64 of A and of B, 2 bytes each
-constexpr int kPkBoxes = 65536;       // staging boxes, 32 rows x 32 columns: two per epilogue warp
-constexpr int kPkSmem = kPkStages * kPkStageBytes + kPkBoxes + 512 + 1024;
+// Shared memory: a ring of stages (16 KiB of A and up to 16 KiB of B, a 64-wide
+// K block of one plane) and the boxes through which the epilogue stores.
+constexpr int kPkData = 229376;
+constexpr int kPkSmem = kPkData + 512 + 1024;
+constexpr int kPkMaxStages = 8;
+constexpr int kPkStageA = 16384;
 
 enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
@@ -466,6 +468,13 @@ __host__ __device__ constexpr int pk_epi_warps(int cg, int epi, bool longk)
 {
     return longk || (cg == 1 && epi == kEpiSoftmax) ? 8 : 16;
 }
+// Boxes of 32 rows x 32 columns. 16 warps have two for 16-bit values (an fp32
+// box takes both), 8 warps two of those or one of fp32: the ring gets the rest,
+// which six plane products of fp32 operands need most, three stages at a time.
+__host__ __device__ constexpr int pk_box_bytes(int cg, int epi, bool longk)
+{
+    return epi == kEpiSoftmax ? 0 : 4096 * pk_epi_warps(cg, epi, longk);
+}
 __host__ __device__ constexpr int pk_threads(int cg, int epi, bool longk) { return 128 + 32 * pk_epi_warps(cg, epi, longk); }
 // Registers a thread: what the launch gives, and the split after setmaxnreg
 // between the first warpgroup and those of the epilogue. The split never sums
@@ -496,13 +505,23 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
     const uint32_t items0 = call.p[0].items;
     const uint32_t items = items0 + (N == 2 ? call.p[N - 1].items : 0u);
     const long long wait_limit = call.p[0].wait_limit;
+    constexpr int kBoxBytes = pk_box_bytes(CG, EPI, LONG);
+    // Bytes of B that a CTA stages for a K block, and the ring for the widest product.
+    const auto b_bytes_of = [&](const ProductParams& p) -> uint32_t {
+        const int lay = LAY == kAnyLayout ? p.layout : LAY;
+        const uint32_t cols = p.tile_n / CG;
+        return lay == kKK ? cols * 128u : (cols > 64 ? 16384u : 8192u);
+    };
+    uint32_t stage_bytes = kPkStageA + b_bytes_of(call.p[0]);
+    if constexpr (N == 2) stage_bytes = max(stage_bytes, kPkStageA + b_bytes_of(call.p[N - 1]));
+    const uint32_t stages = min(static_cast<uint32_t>(kPkData - kBoxBytes) / stage_bytes, static_cast<uint32_t>(kPkMaxStages));
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stage_base = smem;
-    uint8_t* boxes = smem + kPkStages * kPkStageBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(boxes + kPkBoxes);
-    uint64_t* full = bars;        // [kPkStages] leader: bytes of both CTAs landed
-    uint64_t* empty = bars + 8;   // [kPkStages] both: MMAs that read the stage are done
+    uint8_t* boxes = smem + kPkData - kBoxBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPkData);
+    uint64_t* full = bars;        // [kPkMaxStages] leader: bytes of both CTAs landed
+    uint64_t* empty = bars + 8;   // [kPkMaxStages] both: MMAs that read the stage are done
     uint64_t* tfull = bars + 16;  // [2] both: accumulator ready
     uint64_t* tempty = bars + 18; // [2] leader: accumulator read by the epilogue warps of both CTAs
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
@@ -516,7 +535,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
     const uint32_t units = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPkStages; ++s) {
+        for (int s = 0; s < kPkMaxStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -568,8 +587,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                 const int lay = LAY == kAnyLayout ? p.layout : LAY;
                 const bool a_mn = lay == kMNMN, b_mn = lay != kKK;
                 const uint32_t bn_tile = p.tile_n, bn_cta = bn_tile / CG;  // rows of B that this CTA stages
-                const uint32_t b_bytes = b_mn ? (bn_cta > 64 ? 16384u : 8192u) : bn_cta * 128u;
-                const uint32_t tx = CG * (kPkStageBytes / 2 + b_bytes);
+                const uint32_t tx = CG * (kPkStageA + b_bytes_of(p));
                 const uint32_t planes = p.planes, plane_a = p.plane_a, plane_b = p.plane_b;
                 const Item t = decode_item<EPI>(p, which ? i - items0 : i);
                 const int32_t am = static_cast<int32_t>(t.tm * (128 * CG) + cta * 128);
@@ -588,8 +606,8 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         }
                         ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, wait_limit);
                         if (!ok) break;
-                        uint8_t* sa = stage_base + stage * kPkStageBytes;
-                        uint8_t* sb = sa + kPkStageBytes / 2;
+                        uint8_t* sa = stage_base + stage * stage_bytes;
+                        uint8_t* sb = sa + kPkStageA;
                         if (leader && !(call.p[0].test_mode == 1 && issued == 0)) mbar_arrive_expect_tx(&full[stage], tx);
                         auto load = [&](uint8_t* dst, const CUtensorMap* map, int32_t x, int32_t y) {
                             if constexpr (CG == 2)
@@ -610,7 +628,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                             load(sb, map_b, pb + k, bn);
                         }
                         ++issued;
-                        if (++stage == kPkStages) {
+                        if (++stage == stages) {
                             stage = 0;
                             phase ^= 1;
                         }
@@ -622,9 +640,9 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                 // Copies in flight land before the CTA's memory goes away: the
                 // last use of each stage, a bounded wait each.
                 if (leader) {
-                    for (uint32_t s = 0; s < kPkStages; ++s) {
+                    for (uint32_t s = 0; s < stages; ++s) {
                         if (issued <= s) break;
-                        const uint32_t uses = (issued - s - 1) / kPkStages;  // 0-based index of its last use
+                        const uint32_t uses = (issued - s - 1) / stages;  // 0-based index of its last use
                         (void)mbar_wait_drain(&full[s], uses & 1, wait_limit / 8);
                     }
                 }
@@ -648,7 +666,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                                        (b_mn ? 1u << 16 : 0u) | ((p.tile_n >> 3) << 17) |
                                        (static_cast<uint32_t>((128 * CG) >> 4) << 24);
                 const uint64_t a0 = a_mn ? umma_desc_mn_sw128(s0) : umma_desc_sw128(s0);
-                const uint64_t b0 = b_mn ? umma_desc_mn_sw128(s0 + kPkStageBytes / 2) : umma_desc_sw128(s0 + kPkStageBytes / 2);
+                const uint64_t b0 = b_mn ? umma_desc_mn_sw128(s0 + kPkStageA) : umma_desc_sw128(s0 + kPkStageA);
                 const uint64_t ka = a_mn ? 2048 >> 4 : 2;  // 16 of K: 16 rows of 128 bytes, or 32 bytes
                 const uint64_t kb = b_mn ? 2048 >> 4 : 2;
                 const uint32_t planes = p.planes;
@@ -668,15 +686,15 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                         return r;
                     };
                     auto next_stage = [&]() {
-                        if (++stage == kPkStages) {
+                        if (++stage == stages) {
                             stage = 0;
                             phase ^= 1;
                         }
                     };
                     // One K block of stage sa's A against stage sb's B.
                     auto multiply = [&](uint32_t sa, uint32_t sb, bool more) {
-                        const uint64_t ad = a0 + sa * (kPkStageBytes >> 4);
-                        const uint64_t bd = b0 + sb * (kPkStageBytes >> 4);
+                        const uint64_t ad = a0 + sa * (stage_bytes >> 4);
+                        const uint64_t bd = b0 + sb * (stage_bytes >> 4);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const uint32_t add = more || ks > 0 ? 1u : 0u;
@@ -747,26 +765,26 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         constexpr uint32_t kStep = 32 * kGroups;  // columns from one to the next
         int chunks = 0;  // of the current item
         const ProductParams* at_work = &call.p[0];  // the current item's product
-        constexpr int kBox = kPkBoxes / EW / 2;
-        uint8_t* box = boxes + e * 2 * kBox;
+        uint8_t* box = boxes + e * 4096;
         uint32_t nbox = 0;  // boxes sent: picks the buffer
         const uint32_t tempty_leader = CG == 2 ? mapa_shared(smem_u32(tempty), 0u) : 0u;
         const uint32_t lane_base = tmem_base + ((quarter * 32u) << 16) + group * 32;
         uint32_t acc = 0;
         bool ok = true;
 
-        // The buffer of the next box, once the store that read it is done. Two
-        // take turns; an fp32 box of 4 KiB may need the room of both.
+        // The buffer of the next box, once the store that read it is done: two
+        // 16-bit boxes take turns, an fp32 box takes the room of both.
+        bool whole = false;  // the last box did
         auto next_box = [&](bool f32 = false) -> uint8_t* {
-            const bool one = kBox < 4096 && f32;
-            uint8_t* b = box + (one ? 0u : (nbox & 1u) * kBox);
+            uint8_t* b = box + (f32 ? 0u : (nbox & 1u) * 2048u);
             ++nbox;
             if (lane == 0) {
-                if (one)
+                if (f32 || whole)
                     bulk_wait_read<0>();
                 else
                     bulk_wait_read<1>();
             }
+            whole = f32;
             __syncwarp();
             return b;
         };
@@ -989,7 +1007,7 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
                                 if (col + j < p.n) v[j] += load_elem(p.residual, at + j, p.aux_type);
                         }
                     }
-                    uint8_t* b = next_box(p.out_type == kF32 || p.aux_type == kF32);
+                    uint8_t* b = next_box(p.out_type == kF32);
                     if (p.out_type == kF32) {
                         put_f32(b, v);
                     } else {
