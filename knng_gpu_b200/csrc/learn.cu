@@ -288,17 +288,24 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
 // once, at 128 bytes a cycle: single tiles and narrow ones are bound by that. A
 // split product is written and read in fp32 once more, some 3400 bytes a
 // cycle, and may need another kernel to join it.
-double plan_cycles(const Plan& q, const Shape& s)
+double block_cycles(const Plan& q, const Shape& s)
+{
+    const double planes = s.combos == 1 ? 1.0 : 3.0;
+    const double bytes = 16384.0 + 128.0 * q.tile_n / q.cg;
+    return std::max({2.0 * s.combos * q.tile_n, (planes + s.combos) * bytes / 128.0, planes * bytes / 60.0});
+}
+
+// Exponentials of a tile, 16 a cycle.
+double exp_cycles(const Plan& q) { return 128.0 * q.tile_n / 16.0; }
+
+double plan_cycles(const Plan& q, const Shape& s, bool exps = false)
 {
     const uint64_t units = sm_count() / q.cg;
     const uint64_t items = uint64_t(q.tiles_m) * q.tiles_n * q.splits;
     const double rounds = static_cast<double>(ceil_div(items, units));
-    const double planes = s.combos == 1 ? 1.0 : 3.0;
-    const double bytes = 16384.0 + 128.0 * q.tile_n / q.cg;
-    const double block =
-        std::max({2.0 * s.combos * q.tile_n, (planes + s.combos) * bytes / 128.0, planes * bytes / 60.0});
-    const double blocks = static_cast<double>(ceil_div(q.pieces(), q.splits)) * q.piece;
-    double cycles = rounds * (blocks * block + 1500.0) + (q.cg == 2 ? 6000.0 : 0.0);
+    double item = static_cast<double>(ceil_div(q.pieces(), q.splits)) * q.piece * block_cycles(q, s);
+    if (exps) item = std::max(item, exp_cycles(q));
+    double cycles = rounds * (item + 1500.0) + (q.cg == 2 ? 6000.0 : 0.0);
     if (q.splits > 1) cycles += 6000.0 + static_cast<double>(s.m) * s.n * q.splits * 8.0 / 3400.0;
     return cycles;
 }
@@ -337,6 +344,18 @@ Plan search_plan(const Shape& s, int only_cg)
     return best;
 }
 
+bool same(const Shape& a, const Shape& b)
+{
+    return a.m == b.m && a.n == b.n && a.k == b.k && a.combos == b.combos && a.precise == b.precise && a.bf16 == b.bf16;
+}
+
+uint64_t shape_key(const Shape& s)
+{
+    const uint64_t key = (s.m * 0x9E3779B97F4A7C15ull + s.n) * 0xC2B2AE3D27D4EB4Full + s.k * 0x165667B19E3779F9ull +
+                         s.combos * 4 + s.precise * 2 + s.bf16;
+    return key ^ (key >> 29);
+}
+
 // The search takes some microseconds of host time: a thread keeps the plans of
 // the shapes it met last. `cg` 1 or 2 asks for that kind of tile, 0 for either.
 Plan plan_product(const Shape& s, int cg = 0)
@@ -347,29 +366,85 @@ Plan plan_product(const Shape& s, int cg = 0)
         Plan q;
     };
     thread_local Entry kept[128] = {};
-    const uint64_t key = (s.m * 0x9E3779B97F4A7C15ull + s.n) * 0xC2B2AE3D27D4EB4Full + s.k * 0x165667B19E3779F9ull +
-                         s.combos * 16 + cg * 4 + s.precise * 2 + s.bf16;
-    Entry& e = kept[(key ^ (key >> 29)) & 127];
-    if (e.s.m != s.m || e.s.n != s.n || e.s.k != s.k || e.s.combos != s.combos || e.s.precise != s.precise ||
-        e.s.bf16 != s.bf16 || e.cg != cg)
-        e = Entry{s, cg, search_plan(s, cg)};
+    Entry& e = kept[(shape_key(s) + cg) & 127];
+    if (!same(e.s, s) || e.cg != cg) e = Entry{s, cg, search_plan(s, cg)};
     return e.q;
 }
+
+// The longest turn of a unit when the items of a, then those of b, are dealt
+// out in a row.
+double merged_cycles(const Plan& a, const Shape& sa, const Plan& b, const Shape& sb)
+{
+    const uint64_t units = sm_count() / a.cg;
+    const uint64_t na = uint64_t(a.tiles_m) * a.tiles_n * a.splits, all = na + uint64_t(b.tiles_m) * b.tiles_n * b.splits;
+    const double ca = static_cast<double>(ceil_div(a.pieces(), a.splits)) * a.piece * block_cycles(a, sa) + 1500.0;
+    const double cb = static_cast<double>(ceil_div(b.pieces(), b.splits)) * b.piece * block_cycles(b, sb) + 1500.0;
+    double longest = 0.0;
+    for (const uint64_t u : {uint64_t(0), na % units, na % units + units - 1, all % units, all % units + units - 1}) {
+        const uint64_t i = u % units;
+        const uint64_t of_a = na / units + (i < na % units), of_all = all / units + (i < all % units);
+        longest = std::max(longest, static_cast<double>(of_a) * ca + static_cast<double>(of_all - of_a) * cb);
+    }
+    if (a.splits > 1) longest += static_cast<double>(sa.m) * sa.n * a.splits * 8.0 / 3400.0;
+    if (b.splits > 1) longest += static_cast<double>(sb.m) * sb.n * b.splits * 8.0 / 3400.0;
+    return longest + (a.cg == 2 ? 6000.0 : 0.0);
+}
+
+struct TwoPlans {
+    Plan a, b;
+    bool merged;
+};
 
 // Plans of two products of one backward pass, and whether they run in one
 // launch: that saves a launch and half-empty rounds where they are short
 // (gradients of 1537 x 960 -> 300: 26.0 -> 23.2 us), and costs a little where
-// they are not (100,000 x 784 -> 1024: 489 -> 505 us).
+// they are not (100,000 x 784 -> 1024: 489 -> 505 us). In one launch the
+// splits are chosen so that the items of both fill the units together.
+TwoPlans search_two(const Shape& a, const Shape& b)
+{
+    TwoPlans r{plan_product(a), plan_product(b), false};
+    if (plan_cycles(r.a, a) + plan_cycles(r.b, b) > 2e5) return r;
+    r.merged = true;
+    double least = 0.0;
+    for (int cg = 2; cg >= 1; --cg) {
+        const Plan qa = plan_product(a, cg), qb = plan_product(b, cg);
+        const uint64_t units = sm_count() / cg;
+        const auto most = [&](const Plan& q, const Shape& s) {
+            const uint64_t tiles = uint64_t(q.tiles_m) * q.tiles_n;
+            return std::max<uint64_t>(1, std::min<uint64_t>(tiles < units ? units / tiles : 1, q.kblocks / ceil_div(4, s.combos)));
+        };
+        const auto cut = [&](const Plan& q, const Shape& s, uint64_t want) {
+            Plan c = tiles_of(s, cg, q.tile_n);
+            c.piece = static_cast<uint32_t>(std::min<uint64_t>(c.piece, ceil_div(c.kblocks, want)));
+            c.splits = static_cast<uint32_t>(std::min<uint64_t>(want, c.pieces()));
+            return c;
+        };
+        for (uint64_t wa = 1; wa <= most(qa, a); ++wa)
+            for (uint64_t wb = 1; wb <= most(qb, b); wb += wb < 4 ? 1 : wb / 2) {
+                const Plan ca = cut(qa, a, wa), cb = cut(qb, b, wb);
+                const double c = merged_cycles(ca, a, cb, b);
+                if (least == 0.0 || c < least) {
+                    least = c;
+                    r.a = ca;
+                    r.b = cb;
+                }
+            }
+    }
+    return r;
+}
+
 bool plan_two(const Shape& a, const Shape& b, Plan* qa, Plan* qb)
 {
-    *qa = plan_product(a);
-    *qb = plan_product(b);
-    if (plan_cycles(*qa, a) + plan_cycles(*qb, b) > 2e5) return false;
-    const Plan a2 = plan_product(a, 2), b2 = plan_product(b, 2), a1 = plan_product(a, 1), b1 = plan_product(b, 1);
-    const bool pairs = plan_cycles(a2, a) + plan_cycles(b2, b) <= plan_cycles(a1, a) + plan_cycles(b1, b);
-    *qa = pairs ? a2 : a1;
-    *qb = pairs ? b2 : b1;
-    return true;
+    struct Entry {
+        Shape a, b;
+        TwoPlans r;
+    };
+    thread_local Entry kept[64] = {};
+    Entry& e = kept[(shape_key(a) * 31 + shape_key(b)) & 63];
+    if (!same(e.a, a) || !same(e.b, b)) e = Entry{a, b, search_two(a, b)};
+    *qa = e.r.a;
+    *qb = e.r.b;
+    return e.r.merged;
 }
 
 // Opts a kernel in to `bytes` of dynamic shared memory, once per device.
@@ -885,22 +960,32 @@ knng_gpu_status check_scale(const char* op, float scale)
     return KNNG_GPU_OK;
 }
 
-// Pieces of the columns per row tile: as many as make the (row tile, piece)
-// items fill one to eight rounds of the units best, counting that the longest
-// piece of a round sets its time.
-uint32_t softmax_segments(const Plan& q)
+// Pairs or single CTAs, and pieces of the columns per row tile: such that the
+// (row tile, piece) items fill one to eight rounds of the units best, counting
+// that the longest piece of a round sets its time.
+struct SoftmaxPlan {
+    Plan q;
+    uint32_t segments;
+};
+
+SoftmaxPlan plan_softmax(const Shape& s)
 {
-    const uint64_t units = sm_count() / q.cg;
-    uint32_t best = 1;
+    SoftmaxPlan best{};
     double least = 0.0;
-    for (uint64_t rounds = 1; rounds <= 8; ++rounds) {
-        const uint32_t seg = static_cast<uint32_t>(
-            std::max<uint64_t>(1, std::min<uint64_t>(q.tiles_n, rounds * units / q.tiles_m)));
-        const double longest = static_cast<double>(ceil_div(q.tiles_n, seg)) + 0.5;
-        const double time = static_cast<double>(ceil_div(uint64_t(seg) * q.tiles_m, units)) * longest;
-        if (least == 0.0 || time < least) {
-            least = time;
-            best = seg;
+    for (int cg = 2; cg >= 1; --cg) {
+        const Plan q = tiles_of(s, cg, 128 * cg);
+        const uint64_t units = sm_count() / cg;
+        const double tile = std::max(q.kblocks * block_cycles(q, s), exp_cycles(q)) + 300.0;
+        for (uint64_t rounds = 1; rounds <= 8; ++rounds) {
+            const uint32_t seg = static_cast<uint32_t>(
+                std::max<uint64_t>(1, std::min<uint64_t>(q.tiles_n, rounds * units / q.tiles_m)));
+            const double longest = static_cast<double>(ceil_div(q.tiles_n, seg));
+            const double turns = static_cast<double>(ceil_div(uint64_t(seg) * q.tiles_m, units));
+            const double time = turns * (longest * tile + 1500.0) + (cg == 2 ? 6000.0 : 0.0);
+            if (least == 0.0 || time < least) {
+                least = time;
+                best = SoftmaxPlan{q, seg};
+            }
         }
     }
     return best;
@@ -920,10 +1005,10 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     // (row tile, piece) items fill the units in whole rounds.
     const bool skinny = is_skinny(x, w, a.dtype);
     const SkinnyPlan sq = plan_skinny(a.n, a.k);
-    Plan q = tiles_of(s, 2, 256);
-    if (s.m <= 128 || uint64_t(q.tiles_m) * q.tiles_n < sm_count() / 2) q = tiles_of(s, 1, 128);
+    const SoftmaxPlan plan = plan_softmax(s);
+    const Plan& q = plan.q;
+    const uint32_t segments = plan.segments;
     KNNG_TRY(check_items(op, q));
-    const uint32_t segments = softmax_segments(q);
     const uint32_t groups = pk_epi_warps(q.cg, kEpiSoftmax, q.pieces() > 1) / 4;
     const uint32_t pieces = skinny ? sq.blocks : groups * segments;
     Carver c(ws);
@@ -989,8 +1074,18 @@ struct GradPlan {
 
 Plan plan_grad_tiles(const Shape& s)
 {
-    const Plan q = tiles_of(s, 2, 256);
-    return uint64_t(q.tiles_m) * q.tiles_n * 2 >= sm_count() * 3ull / 4 ? q : tiles_of(s, 1, 128);
+    Plan best{};
+    double least = 0.0;
+    for (int cg = 2; cg >= 1; --cg)
+        for (uint32_t tile_n = 128 * cg; tile_n >= 64; tile_n -= 64 * cg) {  // 256 and 128, 128 and 64
+            const Plan q = tiles_of(s, cg, tile_n);
+            const double c = plan_cycles(q, s, true);
+            if (least == 0.0 || c < least) {
+                least = c;
+                best = q;
+            }
+        }
+    return best;
 }
 
 // Pieces: as few as their bytes allow, or a few more where that evens out the
@@ -1013,7 +1108,7 @@ GradPlan plan_grad(uint64_t m, uint64_t k, uint64_t n, int dtype)
         p.g = plan_grad_tiles(sg);
         p.merged = plan_two(sx, sw, &p.dx, &p.dw);
         p.dw_last = count > 1 ? plan_product(sl, p.merged ? p.dx.cg : 0) : p.dw;
-        const double c = static_cast<double>(count) * (plan_cycles(p.g, sg) + plan_cycles(p.dx, sx) + plan_cycles(p.dw, sw));
+        const double c = static_cast<double>(count) * (plan_cycles(p.g, sg, true) + plan_cycles(p.dx, sx) + plan_cycles(p.dw, sw));
         if (least == 0.0 || c < least) {
             least = c;
             best = p;
