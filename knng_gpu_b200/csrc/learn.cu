@@ -310,6 +310,17 @@ double plan_cycles(const Plan& q, const Shape& s, bool exps = false)
     return cycles;
 }
 
+// The K loop cut into about `want` splits of equal length, each a whole number
+// of pieces no longer than `whole`.
+Plan cut_k(Plan q, uint32_t whole, uint64_t want)
+{
+    const uint64_t length = ceil_div(q.kblocks, want);
+    const uint64_t per_split = ceil_div(length, whole);
+    q.piece = static_cast<uint32_t>(ceil_div(length, per_split));
+    q.splits = static_cast<uint32_t>(ceil_div(q.pieces(), per_split));
+    return q;
+}
+
 // The cheapest of pairs (256 rows) and single CTAs (128 rows) with tiles from
 // 64 columns up, the K loop whole or cut into 2, 3, 4, 6, 8, ... splits of at
 // least four K blocks: where the tiles leave units idle, up to as many as fill
@@ -321,16 +332,15 @@ Plan search_plan(const Shape& s, int only_cg)
     for (int cg = 2; cg >= 1; --cg) {
         if (only_cg && cg != only_cg) continue;
         for (uint32_t tile_n = 128 * cg; tile_n >= 64u * cg; tile_n -= 32) {
-            Plan q = tiles_of(s, cg, tile_n);
-            const uint32_t whole = q.piece;
+            const Plan uncut = tiles_of(s, cg, tile_n);
+            Plan q = uncut;
             const uint64_t tiles = uint64_t(q.tiles_m) * q.tiles_n;
             const uint64_t units = sm_count() / cg;
             const uint64_t longest = q.kblocks / ceil_div(4, s.combos);
             const uint64_t most = std::max<uint64_t>(
                 1, std::min<uint64_t>(tiles < units ? units / tiles : tiles < 8 * units ? 8 : 1, longest));
             for (uint64_t want = 1;;) {
-                q.piece = static_cast<uint32_t>(std::min<uint64_t>(whole, ceil_div(q.kblocks, want)));
-                q.splits = static_cast<uint32_t>(std::min<uint64_t>(want, q.pieces()));
+                q = cut_k(uncut, uncut.piece, want);
                 const double c = plan_cycles(q, s);
                 if (least == 0.0 || c < least) {
                     least = c;
@@ -413,15 +423,10 @@ TwoPlans search_two(const Shape& a, const Shape& b)
             const uint64_t tiles = uint64_t(q.tiles_m) * q.tiles_n;
             return std::max<uint64_t>(1, std::min<uint64_t>(tiles < units ? units / tiles : 1, q.kblocks / ceil_div(4, s.combos)));
         };
-        const auto cut = [&](const Plan& q, const Shape& s, uint64_t want) {
-            Plan c = tiles_of(s, cg, q.tile_n);
-            c.piece = static_cast<uint32_t>(std::min<uint64_t>(c.piece, ceil_div(c.kblocks, want)));
-            c.splits = static_cast<uint32_t>(std::min<uint64_t>(want, c.pieces()));
-            return c;
-        };
+        const Plan ua = tiles_of(a, cg, qa.tile_n), ub = tiles_of(b, cg, qb.tile_n);
         for (uint64_t wa = 1; wa <= most(qa, a); ++wa)
             for (uint64_t wb = 1; wb <= most(qb, b); wb += wb < 4 ? 1 : wb / 2) {
-                const Plan ca = cut(qa, a, wa), cb = cut(qb, b, wb);
+                const Plan ca = cut_k(ua, ua.piece, wa), cb = cut_k(ub, ub.piece, wb);
                 const double c = merged_cycles(ca, a, cb, b);
                 if (least == 0.0 || c < least) {
                     least = c;
