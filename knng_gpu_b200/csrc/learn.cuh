@@ -198,14 +198,15 @@ __global__ void __launch_bounds__(256) join_softmax_kernel(const float2* __restr
     if (lane == 0) {
         const bool has = load_label(labels, labels_i64, r, classes) >= 0;
         if (!has) {
-            lse[r] = top == -INFINITY ? top : fmaf(top, 0.69314718f, logf(sum));
+            // No finite score: -inf, unless a NaN is among them.
+            lse[r] = top == -INFINITY && sum == 0.0f ? top : fmaf(top, 0.69314718f, logf(sum));
             loss[r] = 0.0f;
         } else {
             const float y = label_dot[r] * scale2;
             if (!(y < top)) {  // also a NaN score
                 const float others = sum == 0.0f ? y - y : log1pf(sum * exp2_approx(top - y));
                 loss[r] = others;
-                lse[r] = y == -INFINITY ? y : fmaf(y, 0.69314718f, others);
+                lse[r] = y == -INFINITY && sum == 0.0f ? y : fmaf(y, 0.69314718f, others);
             } else {
                 const float tail = logf(sum + exp2_approx(y - top));
                 loss[r] = fmaf(top - y, 0.69314718f, tail);

@@ -129,9 +129,14 @@ def _activation(op: str, name: str) -> int:
     return act
 
 
-def _scope(device, stream):
-    """Allocations and launches on the tensors' device and the call's stream."""
+def _scope(device, stream, *inputs):
+    """Allocations and launches on the tensors' device and the call's stream.
+    On another stream than the current one the allocator learns that the
+    inputs are in use there, so that they may be dropped after the call."""
     if stream is not None:
+        for t in inputs:
+            if t is not None:
+                t.record_stream(stream)
         return torch.cuda.stream(stream)
     if device.index != torch.cuda.current_device():
         return torch.cuda.device(device)
@@ -167,7 +172,7 @@ def linear(x, w, bias=None, residual=None, activation="none", out_dtype=None, ou
         ldr = _stride(op, "residual", residual, m, n)
     if out is not None and (out.device != device or (out_dtype is not None and out.dtype != out_dtype)):
         raise InvalidArgument("knng::gpu::linear: out has another dtype or device than asked for")
-    with _scope(device, stream):
+    with _scope(device, stream, x, w, bias, residual, out, workspace):
         if out is None:
             out, ldo = _rows(m, n, out_dtype or x.dtype, device), n
         else:
@@ -194,7 +199,7 @@ def linear_backward(dy, x, w, pre=None, activation="none", need_dx=True, need_dw
     elif act:
         raise InvalidArgument("knng::gpu::linear_backward: pre is needed with an activation")
     device = x.device
-    with _scope(device, stream):
+    with _scope(device, stream, dy, x, w, pre, workspace):
         dx = _rows(m, k, x.dtype, device) if need_dx else None
         dw = _rows(n, k, x.dtype, device) if need_dw else None
         db = torch.empty(n, dtype=x.dtype, device=device) if need_db else None
@@ -211,7 +216,7 @@ def softmax_xent(x, w, labels, scale=1.0, workspace=None, stream=None):
     m, k, n, ldx, ldw, dtype = _operands(op, x, w)
     device = x.device
     y, i64 = _labels(op, labels, m, device)
-    with _scope(device, stream):
+    with _scope(device, stream, x, w, labels, workspace):
         loss = torch.empty_strided((m,), (1,), dtype=torch.float32, device=device)
         lse = torch.empty_strided((m,), (1,), dtype=torch.float32, device=device)
         _XENT.run(device, workspace, m, k, n, x.data_ptr(), ldx, w.data_ptr(), ldw, y, loss.data_ptr(), lse.data_ptr(),
@@ -230,7 +235,7 @@ def softmax_xent_backward(dloss, x, w, labels, lse, scale=1.0, need_dx=True, nee
     y, i64 = _labels(op, labels, m, device)
     at_dloss = _vector(op, "dloss", dloss, m, torch.float32, device)
     at_lse = _vector(op, "lse", lse, m, torch.float32, device)
-    with _scope(device, stream):
+    with _scope(device, stream, dloss, x, w, labels, lse, workspace):
         dx = _rows(m, k, x.dtype, device) if need_dx else None
         dw = _rows(n, k, x.dtype, device) if need_dw else None
         _XENT_BACKWARD.run(device, workspace, m, k, n, at_dloss, x.data_ptr(), ldx, w.data_ptr(), ldw, y, at_lse,

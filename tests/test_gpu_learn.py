@@ -399,3 +399,42 @@ def test_withheld_arrival_times_out_and_results_stay_right(cuda_ok):
     for m in (100, 3000):
         x, w = rows(g, m, 256, BF16), rows(g, 512, 256, BF16)
         check(kg.linear(x, w), *linear64(x, w, None, None, "none", BF16)[0], "out")
+
+
+@pytest.mark.parametrize("m", [3, 300])  # the kernel for few rows, and the product
+def test_nan_scores_reach_loss_and_lse_of_their_row_only(cuda_ok, m):
+    x, w, labels = xent_case(m, 64, 700, BF16, 507)
+    labels[1] = -1
+    clean = kg.softmax_xent(x, w, labels, 6.0)
+    x[:2] = float("nan")
+    loss, lse = kg.softmax_xent(x, w, labels, 6.0)
+    assert loss[0].isnan() and lse[:2].isnan().all() and loss[1] == 0
+    assert torch.equal(loss[2:], clean[0][2:]) and torch.equal(lse[2:], clean[1][2:])
+
+
+def test_inputs_may_be_dropped_after_a_call_on_another_stream(cuda_ok):
+    side = torch.cuda.Stream()
+    g = make_gen(508)
+    w = rows(g, 512, 512, BF16)
+    want, got = [], []
+    for i in range(20):
+        x = rows(g, 4096, 512, BF16)
+        want.append(kg.linear(x, w))
+        side.wait_stream(torch.cuda.current_stream())
+        got.append(kg.linear(x, w, stream=side))
+        del x
+        torch.zeros((4096, 512), device="cuda", dtype=BF16)  # would take x's memory at once
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_merged_products_with_outputs_of_two_widths(cuda_ok):
+    # Short gradients run dx (fp32 pieces) and dw (16-bit rows) in one launch, through the same store boxes.
+    for seed in range(8):
+        x, w, labels = xent_case(700 + 17 * seed, 128, 9000, BF16, 520 + seed)
+        dloss = torch.full((x.shape[0],), 1e-3, device="cuda")
+        lse = xent64(x, w, labels, 9.0)[1][0].float()
+        got = kg.softmax_xent_backward(dloss, x, w, labels, lse, 9.0)
+        for a, (v, b), name in zip(got, xent_backward64(dloss, x, w, labels, lse, 9.0), ("dx", "dw")):
+            check(a, v, b, (name, seed))
