@@ -272,7 +272,8 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
     q.tiles_n = static_cast<uint32_t>(ceil_div(s.n, tile_n));
     q.kblocks = static_cast<uint32_t>(ceil_div(s.k, 64));
     q.splits = 1;
-    q.piece = std::min(q.kblocks, piece_blocks(s));
+    // As few pieces as the longest allows, all about as long.
+    q.piece = static_cast<uint32_t>(ceil_div(q.kblocks, ceil_div(q.kblocks, piece_blocks(s))));
     q.split_rows = uint64_t(q.tiles_m) * 128 * cg;
     q.part_pitch = uint64_t(q.tiles_n) * tile_n;
     return q;
@@ -340,7 +341,7 @@ Plan search_plan(const Shape& s, int only_cg)
             const uint64_t most = std::max<uint64_t>(
                 1, std::min<uint64_t>(tiles < units ? units / tiles : tiles < 8 * units ? 8 : 1, longest));
             for (uint64_t want = 1;;) {
-                q = cut_k(uncut, uncut.piece, want);
+                q = cut_k(uncut, piece_blocks(s), want);
                 const double c = plan_cycles(q, s);
                 if (least == 0.0 || c < least) {
                     least = c;
@@ -426,7 +427,7 @@ TwoPlans search_two(const Shape& a, const Shape& b)
         const Plan ua = tiles_of(a, cg, qa.tile_n), ub = tiles_of(b, cg, qb.tile_n);
         for (uint64_t wa = 1; wa <= most(qa, a); ++wa)
             for (uint64_t wb = 1; wb <= most(qb, b); wb += wb < 4 ? 1 : wb / 2) {
-                const Plan ca = cut_k(ua, ua.piece, wa), cb = cut_k(ub, ub.piece, wb);
+                const Plan ca = cut_k(ua, piece_blocks(a), wa), cb = cut_k(ub, piece_blocks(b), wb);
                 const double c = merged_cycles(ca, a, cb, b);
                 if (least == 0.0 || c < least) {
                     least = c;

@@ -12,7 +12,7 @@
 // eight warps share a row group and cut K between them. Arithmetic is a
 // fraction of what mma.sync offers; the tensor memory would only add latency.
 //
-// Sums leave the tensor cores every 128 of K and are added to nearest in
+// Sums leave the tensor cores every 32 of K and are added to nearest in
 // registers. fp32 operands are multiplied by the fp32 units: at 4 bytes a value
 // of w they keep up with HBM for 16 rows of x. The loads are the same; a
 // thread's sums over its share of K are added over the four threads of a row.
@@ -213,11 +213,11 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                     load_w<TYPE>(p, r0, c, wa[u]);
                     load_w<TYPE>(p, r0 + 8, c, wb[u]);
                 }
-                float part[NT][4] = {};
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const uint32_t s = s0 + u * p.ksplit;
                     if (s >= steps) break;
+                    float part[NT][4] = {};
                     const uint32_t a0[4] = {wa[u][0], wb[u][0], wa[u][1], wb[u][1]};
                     const uint32_t a1[4] = {wa[u][2], wb[u][2], wa[u][3], wb[u][3]};
 #pragma unroll
@@ -226,11 +226,11 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                         mma_16816(part[q], a0, b.x, b.y, TYPE == kBF16);
                         mma_16816(part[q], a1, b.z, b.w, TYPE == kBF16);
                     }
+#pragma unroll
+                    for (int q = 0; q < NT; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[q][j] += part[q][j];
                 }
-#pragma unroll
-                for (int q = 0; q < NT; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[q][j] += part[q][j];
             }
         }
         if (p.ksplit > 1) {

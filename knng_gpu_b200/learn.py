@@ -49,7 +49,7 @@ class _Operator:
         if workspace is None:
             need = self.size(args)
             if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+                workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device)
         stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
         if workspace is None:
             status = self.call(args, None, 0, stream)
