@@ -721,9 +721,9 @@ struct SkinnyPlan {
 
 // Warps: at least eight per SM by cutting K where w has few rows; at most four
 // blocks of eight warps per SM, which then walk over w.
-SkinnyPlan plan_skinny(uint64_t n, uint64_t k)
+SkinnyPlan plan_skinny(uint64_t n, uint64_t k, int dtype)
 {
-    const uint64_t groups = ceil_div(n, 16), steps = ceil_div(k, 32);
+    const uint64_t groups = ceil_div(n, 16), steps = ceil_div(k, skinny_step(dtype == KNNG_DTYPE_F32));
     SkinnyPlan q{1, 1};
     while (q.ksplit < 8 && groups * q.ksplit < sm_count() * 8ull && steps >= 2 * q.ksplit) q.ksplit *= 2;
     q.blocks = static_cast<uint32_t>(std::min<uint64_t>(ceil_div(groups, 8 / q.ksplit), sm_count() * 4ull));
@@ -766,7 +766,8 @@ SkinnyParams skinny_params(const Source& x, const Source& w, int dtype, const Sk
     p.pitch = skinny_pitch(p.k, dtype == KNNG_DTYPE_F32);
     p.ksplit = q.ksplit;
     p.x_vec = tma_rows(x.ptr, x.ld, elem_bytes(dtype));
-    p.w_vec = tma_rows(w.ptr, w.ld, elem_bytes(dtype));
+    const uint32_t e = elem_bytes(dtype);
+    p.w_vec = !tma_rows(w.ptr, w.ld, e) ? 0 : (reinterpret_cast<uintptr_t>(w.ptr) | w.ld * e) % 32 == 0 ? 2 : 1;
     return p;
 }
 
@@ -805,7 +806,7 @@ knng_gpu_status linear_run(const knng_gpu_linear_args& a, void* ws, uint64_t ws_
     if (a.bias) KNNG_TRY(check_matrix(op, "bias", a.bias, 1, a.n, a.n, a.dtype));
     KNNG_TRY(check_workspace(op, ws, ws_bytes, c.at));
     if (skinny) {
-        const SkinnyPlan sq = plan_skinny(a.n, a.k);
+        const SkinnyPlan sq = plan_skinny(a.n, a.k, a.dtype);
         SkinnyParams p = skinny_params(x, w, a.dtype, sq);
         p.bias = a.bias;
         p.residual = a.residual;
@@ -1010,7 +1011,7 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     // Pairs unless they would leave SMs idle; then the columns are cut so that
     // (row tile, piece) items fill the units in whole rounds.
     const bool skinny = is_skinny(x, w, a.dtype);
-    const SkinnyPlan sq = plan_skinny(a.n, a.k);
+    const SkinnyPlan sq = plan_skinny(a.n, a.k, a.dtype);
     const SoftmaxPlan plan = plan_softmax(s);
     const Plan& q = plan.q;
     const uint32_t segments = plan.segments;

@@ -5,9 +5,9 @@
 // large w and by latency on a small one. There is no staging and no pipeline
 // to fill: every warp takes 16 rows of w straight from memory into the
 // registers of mma.sync (w as the 16-row operand, 8 rows of x as columns),
-// 16 bytes of each of two rows per thread and step of 32 in K. Both operands
-// use the same order of K inside a step, so a thread's 16 bytes are its
-// fragments of two MMAs as they lie. Rows that are not 16-byte aligned are
+// 32 bytes of each of two rows per thread and step: four threads read a whole
+// 128-byte line of a row. Both operands use the same order of K inside a step,
+// so a thread's 32 bytes are its fragments of four MMAs as they lie. Rows that are not 16-byte aligned are
 // read element by element; no row is copied first. With few rows of w, up to
 // eight warps share a row group and cut K between them. Arithmetic is a
 // fraction of what mma.sync offers; the tensor memory would only add latency.
@@ -31,7 +31,7 @@ struct SkinnyParams {
     uint32_t m, n, k;
     uint32_t pitch;        // bytes of a row of x in shared memory
     uint32_t ksplit;       // warps of a block that share a group of 16 rows: 1, 2, 4, 8
-    int x_vec, w_vec;      // rows allow 16-byte loads
+    int x_vec, w_vec;      // rows allow 16-byte loads (1), those of w perhaps 32-byte ones (2)
     // store
     const void* bias;
     const void* residual;
@@ -50,12 +50,14 @@ struct SkinnyParams {
     float* label_dot;
 };
 
-// Bytes of a row of x in shared memory: whole steps; for the 16-bit fragments
-// an odd number of 64-byte units, so that eight rows meet no bank twice.
+// Columns of a step: 128 bytes of a row, 32 per thread.
+__host__ __device__ constexpr uint32_t skinny_step(bool f32) { return f32 ? 32u : 64u; }
+
+// Bytes of a row of x in shared memory: whole steps, and for the 16-bit
+// fragments 16 more, so that eight rows meet no bank twice.
 inline uint32_t skinny_pitch(uint32_t k, bool f32)
 {
-    const uint32_t units = (k + 31) / 32;
-    return f32 ? units * 128 : (units | 1u) * 64;
+    return (k + skinny_step(f32) - 1) / skinny_step(f32) * 128 + (f32 ? 0 : 16);
 }
 
 __device__ __forceinline__ void mma_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1, bool bf16)
@@ -102,11 +104,23 @@ __device__ __forceinline__ void load8_words(const void* src, uint64_t at, uint32
     }
 }
 
-// Columns c .. c + 7 of a row of w.
+// A thread's 32 bytes of a row of w: columns c .. c + 7 of fp32, c .. c + 15 of
+// 16 bits. One instruction where rows lie on 32-byte boundaries.
 template <int TYPE>
 __device__ __forceinline__ void load_w(const SkinnyParams& p, uint32_t row, uint32_t c, uint32_t* out)
 {
-    load8_words<TYPE>(p.w, row * p.ldw + c, row < p.n && c < p.k ? p.k - c : 0u, p.w_vec, out);
+    constexpr uint32_t kValues = TYPE == kF32 ? 8 : 16;
+    const uint64_t at = row * p.ldw + c;
+    const uint32_t left = row < p.n && c < p.k ? p.k - c : 0u;
+    if (p.w_vec == 2 && left >= kValues) {
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(out[0]), "=r"(out[1]), "=r"(out[2]), "=r"(out[3]), "=r"(out[4]), "=r"(out[5]), "=r"(out[6]),
+                       "=r"(out[7])
+                     : "l"(static_cast<const uint8_t*>(p.w) + at * (TYPE == kF32 ? 4 : 2)));
+    } else {
+        load8_words<TYPE>(p.w, at, left, p.w_vec != 0, out);
+        if constexpr (TYPE != kF32) load8_words<TYPE>(p.w, at + 8, left > 8 ? left - 8 : 0u, p.w_vec != 0, out + 4);
+    }
 }
 
 // NT: tiles of 8 rows of x.
@@ -140,7 +154,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
     const uint32_t ks = warp % p.ksplit;
     const uint32_t per_block = 8 / p.ksplit;  // row groups of a block at a time
     const uint32_t groups = (p.n + 15) / 16;
-    const uint32_t steps = (p.k + 31) / 32;
+    const uint32_t steps = (p.k + skinny_step(TYPE == kF32) - 1) / skinny_step(TYPE == kF32);
     // Rounds of the block: every warp takes part in the barriers of each.
     const uint32_t rounds = (groups + per_block - 1) / per_block;
 
@@ -205,31 +219,35 @@ __global__ void __launch_bounds__(256) skinny_kernel(const SkinnyParams p)
                 }
             }
         } else {
-            for (uint32_t s0 = ks; s0 < steps; s0 += 4 * p.ksplit) {
-                uint32_t wa[4][4], wb[4][4];
+            for (uint32_t s0 = ks; s0 < steps; s0 += 2 * p.ksplit) {
+                uint32_t wa[2][8], wb[2][8];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const uint32_t c = (s0 + u * p.ksplit) * 32 + t * 8;
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t c = (s0 + u * p.ksplit) * 64 + t * 16;
                     load_w<TYPE>(p, r0, c, wa[u]);
                     load_w<TYPE>(p, r0 + 8, c, wb[u]);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < 2; ++u) {
                     const uint32_t s = s0 + u * p.ksplit;
                     if (s >= steps) break;
-                    float part[NT][4] = {};
-                    const uint32_t a0[4] = {wa[u][0], wb[u][0], wa[u][1], wb[u][1]};
-                    const uint32_t a1[4] = {wa[u][2], wb[u][2], wa[u][3], wb[u][3]};
 #pragma unroll
-                    for (int q = 0; q < NT; ++q) {
-                        const uint4 b = *reinterpret_cast<const uint4*>(xs + (q * 8 + g) * p.pitch + s * 64 + t * 16);
-                        mma_16816(part[q], a0, b.x, b.y, TYPE == kBF16);
-                        mma_16816(part[q], a1, b.z, b.w, TYPE == kBF16);
+                    for (int h = 0; h < 2; ++h) {
+                        float part[NT][4] = {};
+                        const uint32_t a0[4] = {wa[u][4 * h], wb[u][4 * h], wa[u][4 * h + 1], wb[u][4 * h + 1]};
+                        const uint32_t a1[4] = {wa[u][4 * h + 2], wb[u][4 * h + 2], wa[u][4 * h + 3], wb[u][4 * h + 3]};
+#pragma unroll
+                        for (int q = 0; q < NT; ++q) {
+                            const uint4 b =
+                                *reinterpret_cast<const uint4*>(xs + (q * 8 + g) * p.pitch + s * 128 + t * 32 + h * 16);
+                            mma_16816(part[q], a0, b.x, b.y, TYPE == kBF16);
+                            mma_16816(part[q], a1, b.z, b.w, TYPE == kBF16);
+                        }
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[q][j] += part[q][j];
                     }
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[q][j] += part[q][j];
                 }
             }
         }
