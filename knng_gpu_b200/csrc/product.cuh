@@ -386,15 +386,17 @@ __device__ __forceinline__ void add_words(float* v, const uint4* src, int type)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const float2 f = unpack2(w[j], kBF16);
-            v[2 * j] += f.x;
-            v[2 * j + 1] += f.y;
+            const float2 r = unpair_f32(add2(pair_f32(v[2 * j], v[2 * j + 1]), pair_f32(f.x, f.y)));
+            v[2 * j] = r.x;
+            v[2 * j + 1] = r.y;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const float2 f = unpack2(w[j], kF16);
-            v[2 * j] += f.x;
-            v[2 * j + 1] += f.y;
+            const float2 r = unpair_f32(add2(pair_f32(v[2 * j], v[2 * j + 1]), pair_f32(f.x, f.y)));
+            v[2 * j] = r.x;
+            v[2 * j + 1] = r.y;
         }
     }
 }
