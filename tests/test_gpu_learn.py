@@ -438,3 +438,37 @@ def test_merged_products_with_outputs_of_two_widths(cuda_ok):
         got = kg.softmax_xent_backward(dloss, x, w, labels, lse, 9.0)
         for a, (v, b), name in zip(got, xent_backward64(dloss, x, w, labels, lse, 9.0), ("dx", "dw")):
             check(a, v, b, (name, seed))
+
+
+def test_offsets_beyond_32_bits(cuda_ok):
+    # Matrices of more than 2^31 elements: the last rows have to be right.
+    g = make_gen(700)
+    m, k, n = 2_200_000, 1000, 40
+    x = torch.empty((m, k), device="cuda", dtype=BF16)
+    x.normal_(generator=g)
+    w = rows(g, n, k, BF16, 0, k ** -0.5)
+    tail = slice(m - 300, m)
+    out = kg.linear(x, w, activation="relu")
+    check(out[tail], *linear64(x[tail], w, None, None, "relu", BF16)[0], "linear")
+    dy = rows(g, m, n, BF16, 0, 0.1)
+    dx, _, _ = kg.linear_backward(dy, x, w, need_dw=False)
+    check(dx[tail], *linear_backward64(dy[tail], x[tail], w, None, "none")[0], "dx")
+    del out, dy, dx
+    # The same matrix as the base rows of the loss.
+    labels = torch.tensor([0, m - 1, m - 2, -1], device="cuda")
+    few = rows(g, 4, k, BF16, 0, 0.05)
+    loss, lse = kg.softmax_xent(few, x, labels, 0.5)
+    z = 0.5 * torch.cat([few.double() @ part.double().t() for part in x.split(200_000)], 1)
+    want = torch.logsumexp(z, 1)
+    assert torch.allclose(lse.double(), want, atol=2e-5, rtol=0)
+    at = labels.clamp_min(0)[:, None]
+    assert torch.allclose(loss.double(), (want - z.gather(1, at)[:, 0]) * (labels >= 0), atol=4e-5, rtol=0)
+    dloss = torch.ones(4, device="cuda")
+    _, dw = kg.softmax_xent_backward(dloss, few, x, labels, lse, 0.5, need_dx=False)
+    p = torch.exp(z - lse.double()[:, None])
+    p[torch.arange(3), labels[:3]] -= 1.0
+    p[3] = 0
+    want = 0.5 * p[:, tail].t() @ few.double()
+    # Rounding of g (bf16, 2^-8) and of the result, and the scores' own error.
+    bound = 2.0 ** -7 * (0.5 * p[:, tail].abs().t() @ few.double().abs()) + 2.0 ** -8 * want.abs()
+    check(dw[tail], want, bound + 1e-12, "dw")
