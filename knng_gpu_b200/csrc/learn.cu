@@ -408,13 +408,18 @@ struct TwoPlans {
 
 // Plans of two products of one backward pass, and whether they run in one
 // launch: that saves a launch and half-empty rounds where they are short
-// (gradients of 1537 x 960 -> 300: 26.0 -> 23.2 us), and costs a little where
-// they are not (100,000 x 784 -> 1024: 489 -> 505 us). In one launch the
-// splits are chosen so that the items of both fill the units together.
+// (gradients of 1537 x 960 -> 300: 26.0 -> 23.2 us, of the loss of 4000 x 500
+// against 8000: 141 -> 118 us). Not where they are long (100,000 x 784 -> 1024:
+// 489 -> 505 us), and earlier not where only one of them sums a long K: the
+// other would share its eight epilogue warps instead of having sixteen
+// (100,000 x 784 -> 256: 129 -> 147 us, with odd rows of 785 242 -> 424). In one
+// launch the splits are chosen so that the items of both fill the units
+// together.
 TwoPlans search_two(const Shape& a, const Shape& b)
 {
     TwoPlans r{plan_product(a), plan_product(b), false};
-    if (plan_cycles(r.a, a) + plan_cycles(r.b, b) > 2e5) return r;
+    const bool alike = (r.a.pieces() > r.a.splits) == (r.b.pieces() > r.b.splits);
+    if (plan_cycles(r.a, a) + plan_cycles(r.b, b) > (alike ? 2e5 : 6e4)) return r;
     r.merged = true;
     double least = 0.0;
     for (int cg = 2; cg >= 1; --cg) {

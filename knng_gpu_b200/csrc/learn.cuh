@@ -40,6 +40,19 @@ __device__ void stage_rows(const StageJob& p, uint32_t block)
             if (keep && c0 + 8 <= p.k && (reinterpret_cast<uintptr_t>(src + c0) & 15) == 0) {
                 const uint4 q = *reinterpret_cast<const uint4*>(src + c0);
                 w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+            } else if (keep && c0 + 8 <= p.k && r > 0 && r + 1 < p.rows) {
+                // Whole words, shifted by half a word where the row starts on
+                // one; what they hold beside the eight values lies between the
+                // first and the last row, so it is there to be read.
+                const uintptr_t at = reinterpret_cast<uintptr_t>(src + c0);
+                const uint32_t* word = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+                uint32_t v[5];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = word[j];
+                const bool odd = at & 2;
+                v[4] = odd ? word[4] : 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = odd ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {

@@ -829,16 +829,32 @@ __global__ void __launch_bounds__(pk_threads(CG, EPI, LONG), 1)
         auto copy_out = [&](const uint8_t* b, void* dst, uint64_t ld, int esize, uint32_t row0, uint32_t col0) {
             const ProductParams& p = *at_work;
             __syncwarp();
-            const uint32_t rows = row0 < p.m ? min(32u, p.m - row0) : 0u;
+            const int rows = row0 < p.m ? static_cast<int>(min(32u, p.m - row0)) : 0;
             if (col0 + lane < p.n) {
-                for (uint32_t r = 0; r < rows; ++r) {
-                    const uint64_t at = (row0 + r) * ld + col0 + lane;
-                    if (esize == 2)
-                        static_cast<uint16_t*>(dst)[at] = *reinterpret_cast<const uint16_t*>(
-                            b + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-                    else
-                        static_cast<uint32_t*>(dst)[at] = *reinterpret_cast<const uint32_t*>(
-                            b + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                // A row at a time over the lanes, eight rows in flight.
+                const uint64_t first = row0 * ld + col0 + lane;
+#pragma unroll 1
+                for (int r = 0; r < rows; r += 8) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int q = r + i;  // rows past the last hold values too, only nobody stores them
+                        if (esize == 2)
+                            v[i] = *reinterpret_cast<const uint16_t*>(
+                                b + q * 64 + (((lane >> 3) ^ ((q >> 1) & 3)) << 4) + (lane & 7) * 2);
+                        else
+                            v[i] = *reinterpret_cast<const uint32_t*>(
+                                b + q * 128 + (((lane >> 2) ^ (q & 7)) << 4) + (lane & 3) * 4);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (r + i >= rows) break;
+                        const uint64_t at = first + (r + i) * ld;
+                        if (esize == 2)
+                            static_cast<uint16_t*>(dst)[at] = static_cast<uint16_t>(v[i]);
+                        else
+                            static_cast<uint32_t*>(dst)[at] = v[i];
+                    }
                 }
             }
             __syncwarp();
