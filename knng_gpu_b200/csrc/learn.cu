@@ -1017,12 +1017,12 @@ knng_gpu_status softmax_xent_run(const knng_gpu_softmax_xent_args& a, void* ws, 
     // (row tile, piece) items fill the units in whole rounds.
     const bool skinny = is_skinny(x, w, a.dtype);
     const SkinnyPlan sq = plan_skinny(a.n, a.k, a.dtype);
-    const SoftmaxPlan plan = plan_softmax(s);
+    const SoftmaxPlan plan = skinny ? SoftmaxPlan{} : plan_softmax(s);
     const Plan& q = plan.q;
     const uint32_t segments = plan.segments;
     KNNG_TRY(check_items(op, q));
-    const uint32_t groups = pk_epi_warps(q.cg, kEpiSoftmax, q.pieces() > 1) / 4;
-    const uint32_t pieces = skinny ? sq.blocks : groups * segments;
+    const uint32_t pieces =
+        skinny ? sq.blocks : segments * (pk_epi_warps(q.cg, kEpiSoftmax, q.pieces() > 1) / 4);
     Carver c(ws);
     uint16_t* xs = !skinny && needs_stage(x, a.dtype) ? c.take<uint16_t>(stage_elems(x, a.dtype)) : nullptr;
     uint16_t* wst = !skinny && needs_stage(w, a.dtype) ? c.take<uint16_t>(stage_elems(w, a.dtype)) : nullptr;

@@ -17,8 +17,8 @@
 // Tile and roles. CG = 2: a CTA pair computes up to 256 x 256 with
 // tcgen05.mma.cta_group::2; each CTA stages 128 rows of A and half the tile's
 // rows of B per 64-wide K block, half of what two single-CTA tiles would read
-// from L2. CG = 1: up to 128 x 128 by one CTA, for products with too few tiles to fill the
-// GPU with pairs. Per CTA:
+// from L2. CG = 1: up to 128 x 128 by one CTA, for products with too few tiles
+// to fill the GPU with pairs. Per CTA:
 //   warp 0      TMA producer: as many stages as fit, 5 to 8
 //   warp 1      TMEM allocation; UMMA issue (leader CTA, one lane)
 //   warps 2-3   idle
