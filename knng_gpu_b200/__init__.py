@@ -39,5 +39,6 @@ def __getattr__(name: str):
     if name in _LEARN:
         from . import learn
 
-        return getattr(learn, name)
+        globals().update({n: getattr(learn, n) for n in _LEARN})
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
