@@ -285,15 +285,19 @@ Plan tiles_of(const Shape& s, int cg, uint32_t tile_n)
 // A K block costs the tensor cores 2 cycles per column of the tile (a pair
 // does 256 rows at once, a single CTA 128) and plane product. Its 16 KiB of A
 // and 128 bytes per row of B, for each plane, come from L2 at about 60 bytes a
-// cycle and go into shared memory, from where every plane product reads them
-// once, at 128 bytes a cycle: single tiles and narrow ones are bound by that. A
-// split product is written and read in fp32 once more, some 3400 bytes a
-// cycle, and may need another kernel to join it.
+// cycle and go into shared memory, from where every product reads its share at
+// 128 bytes a cycle (six plane products: A and all of the tile's B each time, a
+// pair's other half from its peer): single tiles and narrow ones are bound by
+// that. A split product is written and read in fp32 once more, some 3400 bytes
+// a cycle, and may need another kernel to join it.
 double block_cycles(const Plan& q, const Shape& s)
 {
     const double planes = s.combos == 1 ? 1.0 : 3.0;
-    const double bytes = 16384.0 + 128.0 * q.tile_n / q.cg;
-    return std::max({2.0 * s.combos * q.tile_n, (planes + s.combos) * bytes / 128.0, planes * bytes / 60.0});
+    const double in = planes * (16384.0 + 128.0 * q.tile_n / q.cg);
+    const double read = s.combos * (16384.0 + 128.0 * q.tile_n);
+    const double l2 = in / 60.0;
+    if (s.combos == 1) return std::max({2.0 * q.tile_n, 2.0 * in / 128.0, l2});
+    return std::max({2.0 * s.combos * q.tile_n, (in + read) / 128.0, l2});
 }
 
 // Exponentials of a tile, 16 a cycle.
