@@ -711,17 +711,23 @@ knng_gpu_status check_workspace(const char* op, const void* ws, uint64_t have, u
 // Few rows of x go to the skinny kernel, its shared memory permitting. Against
 // the product kernel (padded to 128 rows), a linear layer of 16 bf16 rows takes
 // 6.3 us instead of 7.2 at 960 -> 1024 and the same 45 us at 960 -> 100,000,
-// one of 8 rows 4.4 and 38 us. Rows that would have to be staged first (fp16
-// 33 x 785 -> 300: 8.0 us instead of 10.9, in one launch instead of two or
-// three) go there up to 64, sixteen to a block, while w is small enough to be
-// read several times from L2.
+// one of 8 rows 4.4 and 38 us. Operands that would have to be staged first go
+// there, sixteen rows to a block, while that is cheaper than the launch and the
+// copy: up to 64 rows while w is small enough to be read several times from L2
+// (fp16 33 x 785 -> 300: 8.0 us instead of 10.9), and up to 2^24 products (bf16
+// 2000 x 61 -> 100: 4.9 us instead of 6.2, but 15.4 instead of 9.5 at 4e7), of
+// fp32 rows, which the slower units multiply, for 256 of them (100 x 300 -> 300:
+// 7.3 us instead of 11.0; 5000 x 64 -> 64 would take 10.4 instead of 7.4).
 bool is_skinny(const Source& x, const Source& w, int dtype)
 {
     if (x.k > kMaxWidth / 2 || up(std::min<uint64_t>(x.rows, kSkinnyRows), 8) *
                                        skinny_pitch(static_cast<uint32_t>(x.k), dtype == KNNG_DTYPE_F32) > kSkinnySmem)
         return false;
     if (x.rows <= kSkinnyRows) return true;
-    return x.rows <= 4 * kSkinnyRows && w.rows * w.k <= (2ull << 20) && (needs_stage(x, dtype) || needs_stage(w, dtype));
+    if (x.rows > kSkinnyRows * 65535ull || !(needs_stage(x, dtype) || needs_stage(w, dtype))) return false;
+    if (x.rows <= 4 * kSkinnyRows && w.rows * w.k <= (2ull << 20)) return true;
+    return (dtype != KNNG_DTYPE_F32 || x.rows <= 256) &&
+           static_cast<double>(x.rows) * static_cast<double>(w.rows) * static_cast<double>(x.k) <= 16777216.0;
 }
 
 struct SkinnyPlan {
