@@ -716,8 +716,10 @@ knng_gpu_status check_workspace(const char* op, const void* ws, uint64_t have, u
 // copy: up to 64 rows while w is small enough to be read several times from L2
 // (fp16 33 x 785 -> 300: 8.0 us instead of 10.9), and up to 2^24 products (bf16
 // 2000 x 61 -> 100: 4.9 us instead of 6.2, but 15.4 instead of 9.5 at 4e7), of
-// fp32 rows, which the slower units multiply, for 256 of them (100 x 300 -> 300:
-// 7.3 us instead of 11.0; 5000 x 64 -> 64 would take 10.4 instead of 7.4).
+// fp32 rows for 256 of them (100 x 300 -> 300: 7.3 us instead of 11.0). The 256
+// is no crossing point: 1000 x 100 -> 100 would take 6.4 us instead of 8.6, and
+// only near 2e7 products is it slower (5000 x 64 -> 64: 10.4 instead of 7.4). It
+// keeps the product kernel, and a workspace, for fp32 calls of a few hundred rows.
 bool is_skinny(const Source& x, const Source& w, int dtype)
 {
     if (x.k > kMaxWidth / 2 || up(std::min<uint64_t>(x.rows, kSkinnyRows), 8) *
